@@ -504,7 +504,7 @@ __global__ __launch_bounds__(512) void ppg_resident_kernel(PrK a) {
       for (int mm = 0; mm < 5; ++mm) { wm[mm] = s_mix[mm]; isg[mm] = s_mix[16 + mm]; mum[mm] = s_mix[32 + mm]; }
       PR_MARK(4, 2);
       typedef float f32x2 __attribute__((ext_vector_type(2)));
-      f32x2 acc01 = {0.f, 0.f}, acc23 = {0.f, 0.f};  // this wave's share of context = alpha . memory   :115 (v_pk_fma_f32)
+      f32x2 acc01 = {0.f, 0.f}, acc23 = {0.f, 0.f};  // this wave's share of context = alpha . memory   :115
       float* al = a.align_out + (size_t)s * T;
       for (int t0 = wave * NR; t0 < T; t0 += 8 * NR) {  // (one pass up to T_enc = 256)
         // alpha_full[j] = sum_m w_m / (1 + sigmoid((mu_m - (j + 0.5)) / sigma_m))   :101-107, at j = t0 + lane (33 of them matter).
