@@ -764,6 +764,70 @@ int mb_wave_finish_batch(const float* d_wav, const long long* d_pieces, int n_pi
                          double normalize_target, int pcm_mode, void* d_out, void* d_workspace, size_t workspace_bytes,
                          mb_stream_t stream);
 
+/* ----------------------------------------------------------------------
+ * 8. State-space decoder blocks: short causal convolution, selective scan and the norms around a block (csrc/ssm_*.hip).
+ *    The recurrent layer beside the GRU / LSTM loops of sections 3, 4 and 6 for models that replace them; the reference has no such
+ *    layer, so there is no reference interface to cite.  Inference only: nothing here has a backward pass.
+ *
+ *    Types: MB_F32, MB_F16 or MB_BF16 (`dtype`) for activations; parameters, scan states and every sum are fp32.
+ *    Rows: activations are time-major rows with a row stride (elements), dense within a row.  Two forms:
+ *      packed   d_cu_seqlens != NULL: int32 [batch + 1], item b is the rows cu[b] .. cu[b+1]-1 of one [t] row axis (t = rows in all);
+ *      padded   d_cu_seqlens == NULL: [batch][t] rows with a batch stride; item b is its first d_valid[b] rows (NULL: all t).
+ *    Row numbers are read on the device: values outside 0..t are taken as 0 or t.  Rows that belong to no item are left as they were.
+ *    State pools: [n_slots] states, item b owns slot d_slots[b] (NULL: slot b).  An item whose slot is outside 0..n_slots-1, or is named
+ *    by an earlier item of the call too, is left out: neither its rows nor a state are written.  d_has_state[b] == 0: the item starts from
+ *    zeros whatever its slot holds (NULL: every item continues).  A state is updated in place, also that of an item without rows.
+ *    All calls only enqueue kernels on `stream` and may be captured into a graph.
+ * ---------------------------------------------------------------------- */
+#define MB_BF16 3
+
+/* y[t][c] = act(bias[c] + sum_j w[c][j] * x[t - ksize + 1 + j][c]); rows before an item's first one are its state's. */
+typedef struct mb_causal_conv1d_args {
+  const void* d_x;           /* rows of [channels]                                             */
+  void* d_y;                 /* rows of [channels], must not overlap x                         */
+  const float* d_w;          /* fp32 [channels][ksize]                                         */
+  const float* d_bias;       /* fp32 [channels] or NULL                                        */
+  void* d_state;             /* [n_slots][ksize - 1][channels] of `dtype`: the last inputs, oldest first; NULL: none */
+  const int* d_slots; const unsigned char* d_has_state; const int* d_cu_seqlens; const int* d_valid;
+  long long x_bstride, x_rstride, y_bstride, y_rstride, state_stride;  /* elements            */
+  int dtype, batch, t, channels, ksize /* 2..8 */, act /* 0 none, 1 silu */, n_slots;
+} mb_causal_conv1d_args;
+int mb_causal_conv1d(const mb_causal_conv1d_args* a, mb_stream_t stream);
+/* One row per item ([batch] rows of x and y, t / d_cu_seqlens / d_valid / d_has_state unused); d_state is required. */
+int mb_causal_conv1d_step(const mb_causal_conv1d_args* a, mb_stream_t stream);
+
+/* Per head: d = dt + dt_bias, through softplus if asked for, clamped to [dt_min, dt_max]; h = exp(d * A) * h + (d * x) B^T; y = h C + D * x.
+ * x, y: rows of [heads][head_dim]; dt: rows of [heads]; B, C: rows of [groups][d_state], head i reads group i / (heads / groups). */
+typedef struct mb_selective_scan_args {
+  const void* d_x; void* d_y; /* must not overlap any input                                    */
+  const void* d_dt; const void* d_b; const void* d_c;
+  const float* d_a; const float* d_d; const float* d_dt_bias;  /* fp32 [heads]; d_d, d_dt_bias may be NULL */
+  float* d_state;             /* fp32 [n_slots][heads][head_dim][d_state] or NULL              */
+  const int* d_slots; const unsigned char* d_has_state; const int* d_cu_seqlens; const int* d_valid;
+  long long x_bstride, x_rstride, y_bstride, y_rstride, dt_bstride, dt_rstride, b_bstride, b_rstride, c_bstride, c_rstride, state_stride;
+  int dtype, dt_dtype /* dtype or MB_F32 */, batch, t, heads, head_dim /* 1..128 */, groups, d_state_dim /* 1..256 */, n_slots;
+  int dt_softplus; float dt_min, dt_max;
+} mb_selective_scan_args;
+size_t mb_selective_scan_workspace_bytes(const mb_selective_scan_args* a);
+int mb_selective_scan(const mb_selective_scan_args* a, void* d_workspace, size_t workspace_bytes, mb_stream_t stream);
+/* One row per item, no workspace; d_state is required. */
+int mb_selective_scan_step(const mb_selective_scan_args* a, mb_stream_t stream);
+
+/* The seam between two blocks, per row of [channels]:
+ *   u = x * act(gate) if gate_first;  v = norm(u);  v *= act(gate) if not gate_first;  s = residual + scale * v;  y = next_norm(s).
+ * norm / next_norm: 0 none, 1 RMS, 2 layer norm (weight and bias NULL: ones and zeros); `groups`: the first norm over each of that many
+ * equal parts of the row.  d_gate, d_residual NULL: without; scale = res_scale * d_scale[c] (NULL: 1).  d_sum receives s (NULL: not
+ * stored), d_y the result of next_norm (only with next_norm).  x, gate and y are `dtype`; residual and sum `res_dtype` (dtype or MB_F32).
+ * An output may be exactly one of the inputs, otherwise nothing overlaps. */
+typedef struct mb_block_norm_args {
+  const void* d_x; const void* d_gate; const void* d_residual; void* d_sum; void* d_y;
+  const float* d_weight; const float* d_bias; const float* d_scale; const float* d_next_weight; const float* d_next_bias;  /* fp32 [channels] */
+  long long rows, x_rstride, gate_rstride, residual_rstride, sum_rstride, y_rstride;
+  int dtype, res_dtype, channels, groups, norm, next_norm, gate_act /* 0 none, 1 silu, 2 sigmoid */, gate_first;
+  float eps, next_eps, res_scale;
+} mb_block_norm_args;
+int mb_block_norm(const mb_block_norm_args* a, mb_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -84,7 +84,7 @@ class Ppg2MelConfig(C.Structure):
     ]
 
 
-MB_F32, MB_F16, MB_F64 = 0, 1, 2
+MB_F32, MB_F16, MB_F64, MB_BF16 = 0, 1, 2, 3
 MB_PCM16_SNDFILE, MB_PCM16_ENCODE16, MB_PCM16_SAVE_WAV = 0, 1, 2
 
 
@@ -157,6 +157,30 @@ class TacoConfig(C.Structure):
         ("has_gst", C.c_int), ("gst_tokens", C.c_int), ("gst_heads", C.c_int), ("gst_n_convs", C.c_int),
         ("gst_width", C.c_int), ("gst_filters", C.c_int * 8), ("dropout", C.c_float),
     ]
+
+
+class CausalConv1dArgs(C.Structure):
+    _fields_ = ([(n, C.c_void_p) for n in ("d_x", "d_y", "d_w", "d_bias", "d_state", "d_slots", "d_has_state", "d_cu_seqlens", "d_valid")]
+                + [(n, C.c_longlong) for n in ("x_bstride", "x_rstride", "y_bstride", "y_rstride", "state_stride")]
+                + [(n, C.c_int) for n in ("dtype", "batch", "t", "channels", "ksize", "act", "n_slots")])
+
+
+class SelectiveScanArgs(C.Structure):
+    _fields_ = ([(n, C.c_void_p) for n in ("d_x", "d_y", "d_dt", "d_b", "d_c", "d_a", "d_d", "d_dt_bias", "d_state", "d_slots",
+                                           "d_has_state", "d_cu_seqlens", "d_valid")]
+                + [(n, C.c_longlong) for n in ("x_bstride", "x_rstride", "y_bstride", "y_rstride", "dt_bstride", "dt_rstride", "b_bstride",
+                                               "b_rstride", "c_bstride", "c_rstride", "state_stride")]
+                + [(n, C.c_int) for n in ("dtype", "dt_dtype", "batch", "t", "heads", "head_dim", "groups", "d_state_dim", "n_slots",
+                                          "dt_softplus")]
+                + [("dt_min", C.c_float), ("dt_max", C.c_float)])
+
+
+class BlockNormArgs(C.Structure):
+    _fields_ = ([(n, C.c_void_p) for n in ("d_x", "d_gate", "d_residual", "d_sum", "d_y", "d_weight", "d_bias", "d_scale",
+                                           "d_next_weight", "d_next_bias")]
+                + [(n, C.c_longlong) for n in ("rows", "x_rstride", "gate_rstride", "residual_rstride", "sum_rstride", "y_rstride")]
+                + [(n, C.c_int) for n in ("dtype", "res_dtype", "channels", "groups", "norm", "next_norm", "gate_act", "gate_first")]
+                + [("eps", C.c_float), ("next_eps", C.c_float), ("res_scale", C.c_float)])
 
 
 # name -> (restype, argtypes); must list every symbol include/mbhip.h declares
@@ -289,6 +313,12 @@ SIGNATURES = {
     "mb_taco_encode_workspace_bytes": (C.c_size_t, [C.c_void_p, C.c_int, C.c_int]),
     "mb_taco_encode": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int,
                                  C.c_void_p, C.c_uint64, C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]),
+    "mb_causal_conv1d": (C.c_int, [C.POINTER(CausalConv1dArgs), C.c_void_p]),
+    "mb_causal_conv1d_step": (C.c_int, [C.POINTER(CausalConv1dArgs), C.c_void_p]),
+    "mb_selective_scan_workspace_bytes": (C.c_size_t, [C.POINTER(SelectiveScanArgs)]),
+    "mb_selective_scan": (C.c_int, [C.POINTER(SelectiveScanArgs), C.c_void_p, C.c_size_t, C.c_void_p]),
+    "mb_selective_scan_step": (C.c_int, [C.POINTER(SelectiveScanArgs), C.c_void_p]),
+    "mb_block_norm": (C.c_int, [C.POINTER(BlockNormArgs), C.c_void_p]),
     "mb_maximum_path": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int,
                                   C.c_int, C.c_void_p]),
 }
