@@ -13,7 +13,7 @@ CSRC = ROOT / "csrc"
 LIB = ROOT / "libmbhip.so"
 ARCH = "gfx950"
 SOURCES = ["common.hip", "conv1d.hip", "conv1d_f16.hip", "resblock_f16.hip", "resblock_stage_f16.hip", "resblock_stage_f32.hip", "resblock_pair_split.hip", "conv_split_tm.hip", "gan.hip", "rnn.hip", "wavernn.hip", "wavernn_post.hip", "wave_post.hip", "tacotron.hip", "ppg2mel.hip", "ppg_net.hip",
-           "maximum_path.hip", "ssm_conv.hip", "ssm_scan.hip", "ssm_norm.hip"]
+           "maximum_path.hip", "ssm_conv.hip", "ssm_scan.hip", "ssm_scan_f32.hip", "ssm_scan_f16.hip", "ssm_scan_bf16.hip", "ssm_norm.hip"]
 # packed fp32 arithmetic (v_pk_add_f32 and its like, which -O3 forms by itself from ordinary float code) is switched off: some of its
 # forms have given wrong results on this hardware now and then, without an error.  hipcc's host pass warns that it does not know the feature.
 FLAGS = ["-O3", "-std=c++17", "-fPIC", f"--offload-arch={ARCH}", "-fno-gpu-rdc",

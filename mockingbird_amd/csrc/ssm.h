@@ -85,7 +85,7 @@ __device__ __forceinline__ int slot_of(const int* slots, int b, int n_slots) {
   return __any(twice) ? -1 : s;
 }
 
-static inline bool aligned(const void* p, size_t n) { return ((size_t)p & (n - 1)) == 0; }
+__host__ __device__ static inline bool aligned(const void* p, size_t n) { return ((size_t)p & (n - 1)) == 0; }
 
 }  // namespace ssm
 }  // namespace mb

@@ -1,16 +1,8 @@
 // Selective state space scan: per head a state h [head_dim][d_state] that decays by exp(d A), takes in (d x) B^T and answers y = h C + D x.
-#include "ssm.h"
+#include "ssm_scan_chunk.h"
 
 namespace mb {
 namespace ssm {
-
-// exp and the step sizes are the library's fp32 functions: a decay error of one step is taken to the power of the sequence's length
-__device__ __forceinline__ float step_size(const mb_selective_scan_args& a, long long at, int head) {
-  float d = a.dt_dtype == MB_F32 ? ((const float*)a.d_dt)[at] : a.dt_dtype == MB_F16 ? to_f32(((const f16*)a.d_dt)[at]) : to_f32(((const bf16*)a.d_dt)[at]);
-  if (a.d_dt_bias) d += a.d_dt_bias[head];
-  if (a.dt_softplus) d = softplus(d);
-  return d < a.dt_min ? a.dt_min : d > a.dt_max ? a.dt_max : d;  // NaN stays NaN
-}
 
 // Four state columns n .. n+3 of a row; columns from `left` on do not exist and stay zero.  VEC: rows of whole, 16-byte aligned quads.
 template <bool VEC> __device__ __forceinline__ f32x4 load_quad(const float* p, int left) {
@@ -79,95 +71,92 @@ __global__ __launch_bounds__(256) void selective_scan_step_kernel(const mb_selec
   }
 }
 
-// Row after row: one workgroup per item and head, the head's state in registers (LANES lanes per state row as above).
-template <typename T, int LANES, bool VEC>
-__global__ __launch_bounds__(256) void selective_scan_rows_kernel(const mb_selective_scan_args a) {
-  constexpr int ROWS = 256 / LANES, PASSES = 128 / ROWS > 0 ? 128 / ROWS : 1;
-  const int b = (int)(blockIdx.x / a.heads), head = (int)(blockIdx.x - (unsigned)b * a.heads);
+// Between the two passes of a split call: every tile's own sum becomes the state in front of it.
+__global__ __launch_bounds__(256) void selective_scan_join_kernel(const mb_selective_scan_args a, const Split sp) {
+  const int elems = a.head_dim * a.d_state_dim, blocks = (elems + 255) / 256;
+  const unsigned item_head = blockIdx.x / blocks;
+  const int e = (int)(blockIdx.x - item_head * blocks) * 256 + (int)threadIdx.x;
+  const int b = (int)(item_head / a.heads), head = (int)(item_head - (unsigned)b * a.heads);
   int slot = -1;
   if (a.d_state) {
     slot = slot_of(a.d_slots, b, a.n_slots);
     if (slot < 0) return;
   }
-  long long row = 0;
-  int len = a.t;
+  if (e >= elems) return;
+  long long tile;
+  int len;
   if (a.d_cu_seqlens) {
     const int s = min(max(a.d_cu_seqlens[b], 0), a.t);
-    row = s;
     len = min(max(a.d_cu_seqlens[b + 1], s), a.t) - s;
-  } else if (a.d_valid) {
-    len = min(max(a.d_valid[b], 0), a.t);
+    tile = s / sp.seg + b;
+  } else {
+    len = a.d_valid ? min(max(a.d_valid[b], 0), a.t) : a.t;
+    tile = (long long)b * (a.t > sp.seg ? (a.t + sp.seg - 1) / sp.seg : 1);
   }
-  const long long pad = a.d_cu_seqlens ? 0 : b;
-  const int n = (int)(threadIdx.x % LANES) * 4, left = a.d_state_dim - n, p0 = (int)threadIdx.x / LANES;
-  const int group = head / (a.heads / a.groups);
-  const T* x = (const T*)a.d_x + pad * a.x_bstride + row * a.x_rstride + (long long)head * a.head_dim;
-  T* y = (T*)a.d_y + pad * a.y_bstride + row * a.y_rstride + (long long)head * a.head_dim;
-  const T* bm = (const T*)a.d_b + pad * a.b_bstride + row * a.b_rstride + (long long)group * a.d_state_dim + n;
-  const T* cm = (const T*)a.d_c + pad * a.c_bstride + row * a.c_rstride + (long long)group * a.d_state_dim + n;
-  const long long dt = pad * a.dt_bstride + row * a.dt_rstride + head;
-  float* st = a.d_state ? a.d_state + slot * a.state_stride + (long long)head * a.head_dim * a.d_state_dim + n : nullptr;
-  const bool keep = st && (!a.d_has_state || a.d_has_state[b]);
-  const float A = a.d_a[head], skip = a.d_d ? a.d_d[head] : 0.f;
-  f32x4 h[PASSES];
-#pragma unroll
-  for (int i = 0; i < PASSES; ++i) {
-    const int p = p0 + i * ROWS;
-    h[i] = keep && p < a.head_dim ? load_quad<VEC>(st + (long long)p * a.d_state_dim, left) : f32x4{0.f, 0.f, 0.f, 0.f};
+  const int parts = max(1, (len + sp.seg - 1) / sp.seg);
+  float h = 0.f;
+  if (a.d_state && (!a.d_has_state || a.d_has_state[b])) h = a.d_state[slot * a.state_stride + (long long)head * elems + e];
+  const long long step = (long long)a.heads * elems;
+  float* st = sp.state + (tile * a.heads + head) * (long long)elems + e;
+  const float* decay = sp.decay + tile * a.heads + head;
+  float own = 0.f, next = parts > 1 ? st[0] : 0.f;
+  for (int k = 0; k < parts; ++k) {
+    own = next;
+    if (k + 2 < parts) next = st[step];  // the last tile's own sum is not computed: nothing follows it
+    st[0] = h;
+    if (k + 1 < parts) h = fmaf(h, *decay, own);
+    st += step;
+    decay += a.heads;
   }
-  for (int t = 0; t < len; ++t) {
-    const float d = step_size(a, dt + t * a.dt_rstride, head), decay = expf(d * A);
-    const f32x4 bv = load_quad_of(bm + t * a.b_rstride, left), cv = load_quad_of(cm + t * a.c_rstride, left);
-#pragma unroll
-    for (int i = 0; i < PASSES; ++i) {
-      const int p = p0 + i * ROWS;
-      const float xv = p < a.head_dim ? to_f32(x[t * a.x_rstride + p]) : 0.f, dx = d * xv;
-      float s = 0.f;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        h[i][k] = fmaf(h[i][k], decay, dx * bv[k]);
-        s = fmaf(h[i][k], cv[k], s);
-      }
-      s = lanes_sum<LANES>(s);
-      if (n == 0 && p < a.head_dim) y[t * a.y_rstride + p] = from_f32<T>(fmaf(skip, xv, s));
-    }
-  }
-  if (st)
-#pragma unroll
-    for (int i = 0; i < PASSES; ++i) {
-      const int p = p0 + i * ROWS;
-      if (p < a.head_dim) store_quad<VEC>(st + (long long)p * a.d_state_dim, h[i], left);
-    }
 }
 
-template <typename T, int LANES, bool VEC> int launch_scan(const mb_selective_scan_args& a, bool step, hipStream_t s) {
-  if (step) {
-    constexpr int ROWS = 256 / LANES;
-    int pb = (a.head_dim + ROWS - 1) / ROWS * ROWS;
-    // few requests: a head's rows are dealt to more workgroups, down to one pass each, until two fit every CU
-    while (pb > ROWS && (long long)a.batch * a.heads * ((a.head_dim + pb - 1) / pb) < 512) pb = (pb / ROWS + 1) / 2 * ROWS;
-    const long long grid = (long long)a.batch * a.heads * ((a.head_dim + pb - 1) / pb);
-    MB_REQUIRE(grid < (1ll << 31), "selective_scan_step: %d items of %d heads are too many for one launch", a.batch, a.heads);
-    hipLaunchKernelGGL((selective_scan_step_kernel<T, LANES, VEC>), dim3((unsigned)grid), dim3(256), 0, s, a, pb);
-  } else {
-    MB_REQUIRE((long long)a.batch * a.heads < (1ll << 31), "selective_scan: %d items of %d heads are too many for one launch", a.batch, a.heads);
-    hipLaunchKernelGGL((selective_scan_rows_kernel<T, LANES, VEC>), dim3((unsigned)(a.batch * a.heads)), dim3(256), 0, s, a);
-  }
+template <typename T, int LANES, bool VEC> int launch_step(const mb_selective_scan_args& a, hipStream_t s) {
+  constexpr int ROWS = 256 / LANES;
+  int pb = (a.head_dim + ROWS - 1) / ROWS * ROWS;
+  // few requests: a head's rows are dealt to more workgroups, down to one pass each, until two fit every CU
+  while (pb > ROWS && (long long)a.batch * a.heads * ((a.head_dim + pb - 1) / pb) < 512) pb = (pb / ROWS + 1) / 2 * ROWS;
+  const long long grid = (long long)a.batch * a.heads * ((a.head_dim + pb - 1) / pb);
+  MB_REQUIRE(grid < (1ll << 31), "selective_scan_step: %d items of %d heads are too many for one launch", a.batch, a.heads);
+  hipLaunchKernelGGL((selective_scan_step_kernel<T, LANES, VEC>), dim3((unsigned)grid), dim3(256), 0, s, a, pb);
   MB_HIP(hipGetLastError());
   return MB_OK;
 }
 
-template <typename T, bool VEC> int scan_by_lanes(const mb_selective_scan_args& a, bool step, hipStream_t s) {
-  if (a.d_state_dim <= 16) return launch_scan<T, 4, VEC>(a, step, s);
-  if (a.d_state_dim <= 32) return launch_scan<T, 8, VEC>(a, step, s);
-  if (a.d_state_dim <= 64) return launch_scan<T, 16, VEC>(a, step, s);
-  if (a.d_state_dim <= 128) return launch_scan<T, 32, VEC>(a, step, s);
-  return launch_scan<T, 64, VEC>(a, step, s);
+template <typename T, bool VEC> int step_by_lanes(const mb_selective_scan_args& a, hipStream_t s) {
+  if (a.d_state_dim <= 16) return launch_step<T, 4, VEC>(a, s);
+  if (a.d_state_dim <= 32) return launch_step<T, 8, VEC>(a, s);
+  if (a.d_state_dim <= 64) return launch_step<T, 16, VEC>(a, s);
+  if (a.d_state_dim <= 128) return launch_step<T, 32, VEC>(a, s);
+  return launch_step<T, 64, VEC>(a, s);
 }
 
-template <typename T> int scan_by_width(const mb_selective_scan_args& a, bool step, hipStream_t s) {
-  const bool vec = a.d_state_dim % 4 == 0 && (!a.d_state || (aligned(a.d_state, 16) && a.state_stride % 4 == 0));
-  return vec ? scan_by_lanes<T, true>(a, step, s) : scan_by_lanes<T, false>(a, step, s);
+template <typename T> int step_by_width(const mb_selective_scan_args& a, hipStream_t s) {
+  const bool vec = a.d_state_dim % 4 == 0 && aligned(a.d_state, 16) && a.state_stride % 4 == 0;
+  return vec ? step_by_lanes<T, true>(a, s) : step_by_lanes<T, false>(a, s);
+}
+
+// Rows of a time tile, or 0 for one workgroup walking a whole item.  A tile's workgroups carry units_of() heads' states; about 512
+// workgroups (two per CU) are wanted.  The host does not know the lengths of packed items: it deals out the rows of all together.
+static int rows_per_tile(const mb_selective_scan_args& a) {
+  const int hb = a.dtype == MB_F32 && a.d_state_dim > 128 ? 2 : 4;
+  const long long units = (long long)a.groups * cdiv(a.heads / a.groups, hb) * cdiv(a.head_dim, 64);
+  const long long all = a.d_cu_seqlens ? a.t : (long long)a.t * a.batch;
+  long long seg = (all * units + 511) / 512;
+  if (seg < 256) seg = 256;
+  seg = (seg + 63) / 64 * 64;
+  return seg >= a.t ? 0 : (int)seg;
+}
+
+static size_t split_layout(const mb_selective_scan_args& a, void* base, Split* sp) {
+  sp->seg = rows_per_tile(a);
+  sp->state = sp->decay = nullptr;
+  if (!sp->seg) return 0;
+  const Rows rows = {a.d_cu_seqlens, a.d_valid, a.batch, a.t};
+  const size_t tiles = (size_t)tiles_of(rows, sp->seg);
+  Arena ar(base, ~(size_t)0);
+  sp->state = ar.take<float>(tiles * a.heads * a.head_dim * a.d_state_dim);
+  sp->decay = ar.take<float>(tiles * a.heads);
+  return align_up(ar.off, 256);
 }
 
 static int check_scan(const char* name, const mb_selective_scan_args* a, bool step) {
@@ -194,21 +183,44 @@ static int check_scan(const char* name, const mb_selective_scan_args* a, bool st
   return 1;
 }
 
-static int run_scan(const char* name, const mb_selective_scan_args* a, bool step, mb_stream_t stream) {
-  const int go = check_scan(name, a, step);
+static int run_scan(const mb_selective_scan_args* a, void* ws, size_t ws_bytes, hipStream_t s) {
+  const int go = check_scan("selective_scan", a, false);
   if (go <= 0) return go;
-  if (a->dtype == MB_F32) return scan_by_width<float>(*a, step, (hipStream_t)stream);
-  if (a->dtype == MB_F16) return scan_by_width<f16>(*a, step, (hipStream_t)stream);
-  return scan_by_width<bf16>(*a, step, (hipStream_t)stream);
+  Split sp;
+  const size_t need = split_layout(*a, ws, &sp);
+  if (ws_bytes < need || (need && !ws)) {
+    set_error("selective_scan: workspace of %zu B, %zu B are needed", ws_bytes, need);
+    return MB_ENOMEM;
+  }
+  MB_REQUIRE(aligned(ws, 16), "selective_scan: the workspace must be 16-byte aligned");
+  auto* chunks = a->dtype == MB_F32 ? scan_chunks_f32 : a->dtype == MB_F16 ? scan_chunks_f16 : scan_chunks_bf16;
+  if (sp.seg) {
+    const int rc = chunks(*a, sp, true, s);
+    if (rc) return rc;
+    const long long grid = (long long)a->batch * a->heads * cdiv(a->head_dim * a->d_state_dim, 256);
+    MB_REQUIRE(grid < (1ll << 31), "selective_scan: %d items of %d heads are too many for one launch", a->batch, a->heads);
+    hipLaunchKernelGGL(selective_scan_join_kernel, dim3((unsigned)grid), dim3(256), 0, s, *a, sp);
+    MB_HIP(hipGetLastError());
+  }
+  return chunks(*a, sp, false, s);
+}
+
+static int run_step(const mb_selective_scan_args* a, hipStream_t s) {
+  const int go = check_scan("selective_scan_step", a, true);
+  if (go <= 0) return go;
+  return a->dtype == MB_F32 ? step_by_width<float>(*a, s) : a->dtype == MB_F16 ? step_by_width<f16>(*a, s) : step_by_width<bf16>(*a, s);
 }
 
 }  // namespace ssm
 }  // namespace mb
 
-extern "C" size_t mb_selective_scan_workspace_bytes(const mb_selective_scan_args* a) { return 0; }
+extern "C" size_t mb_selective_scan_workspace_bytes(const mb_selective_scan_args* a) {
+  using namespace mb::ssm;
+  if (!a || a->batch <= 0 || a->heads <= 0 || a->t <= 0 || a->groups <= 0 || a->head_dim <= 0 || a->d_state_dim <= 0) return 0;
+  Split sp;
+  return split_layout(*a, nullptr, &sp);
+}
 extern "C" int mb_selective_scan(const mb_selective_scan_args* a, void* d_workspace, size_t workspace_bytes, mb_stream_t stream) {
-  return mb::ssm::run_scan("selective_scan", a, false, stream);
+  return mb::ssm::run_scan(a, d_workspace, workspace_bytes, (hipStream_t)stream);
 }
-extern "C" int mb_selective_scan_step(const mb_selective_scan_args* a, mb_stream_t stream) {
-  return mb::ssm::run_scan("selective_scan_step", a, true, stream);
-}
+extern "C" int mb_selective_scan_step(const mb_selective_scan_args* a, mb_stream_t stream) { return mb::ssm::run_step(a, (hipStream_t)stream); }
