@@ -13,15 +13,33 @@ typedef _Float16 f16;
 template <typename T> __device__ __forceinline__ float to_f32(T v) { return (float)v; }
 template <typename T> __device__ __forceinline__ T from_f32(float v) { return (T)v; }  // one rounding to nearest even
 
-// N elements as one load / store; the host only picks N > 1 where every pointer and stride keeps N * sizeof(T) bytes aligned
+// N elements as one access.  Rows start at any element (odd widths, slices), so the accesses ask for the element's alignment only: global
+// memory takes a 16-byte access at any address, at the price of the extra cache line it may touch.
 template <typename T, int N> struct Vec { T v[N]; };
 template <typename T, int N> __device__ __forceinline__ Vec<T, N> load_vec(const T* p) {
-  typedef T vt __attribute__((ext_vector_type(N)));
+  typedef T vt __attribute__((ext_vector_type(N), aligned(sizeof(T))));
   return __builtin_bit_cast(Vec<T, N>, *(const vt*)p);
 }
 template <typename T, int N> __device__ __forceinline__ void store_vec(T* p, const Vec<T, N>& v) {
-  typedef T vt __attribute__((ext_vector_type(N)));
+  typedef T vt __attribute__((ext_vector_type(N), aligned(sizeof(T))));
   *(vt*)p = __builtin_bit_cast(vt, v);
+}
+// The first n of N elements (the rest are zero / left alone): the end of a row whose width N does not divide.
+template <typename T, int N> __device__ __forceinline__ Vec<T, N> load_some(const T* p, int n) {
+  Vec<T, N> v;
+  if (n >= N) return load_vec<T, N>(p);
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    v.v[i] = (T)0.f;
+    if (i < n) v.v[i] = p[i];
+  }
+  return v;
+}
+template <typename T, int N> __device__ __forceinline__ void store_some(T* p, const Vec<T, N>& v, int n) {
+  if (n >= N) return store_vec<T, N>(p, v);
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    if (i < n) p[i] = v.v[i];
 }
 
 // exp and 1 / (1 + exp(-v)).  fp32 results go through the library's expf and a full division; a 16-bit result is rounded to 2^-9 or

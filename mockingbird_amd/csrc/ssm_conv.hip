@@ -5,13 +5,35 @@
 namespace mb {
 namespace ssm {
 
-template <typename T, int K, int V>
+// The taps of V channels: one run of V * K floats.
+template <int K, int V> __device__ __forceinline__ void load_taps(const float* w, int n, float (&out)[V][K]) {
+  if (n >= V) {
+    constexpr int Q = V * K / 4;  // V is 4 or 8
+    Vec<float, 4> q[Q];
+#pragma unroll
+    for (int i = 0; i < Q; ++i) q[i] = load_vec<float, 4>(w + 4 * i);
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+#pragma unroll
+      for (int j = 0; j < K; ++j) out[i][j] = q[(i * K + j) / 4].v[(i * K + j) % 4];
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+#pragma unroll
+      for (int j = 0; j < K; ++j) out[i][j] = i < n ? w[i * K + j] : 0.f;
+  }
+}
+
+// A thread takes V channels (16 bytes of them) of R rows, cx threads side by side and 256 / cx runs of R rows behind each other.  Memory-
+// bound: each row is read once (a run reads K - 1 more) and the window slides through registers; U rows are requested at a time.
+template <typename T, int K>
 __global__ __launch_bounds__(256) void causal_conv1d_kernel(const mb_causal_conv1d_args a, int cx, int R) {
   constexpr bool FAST = sizeof(T) == 2;
+  constexpr int V = 16 / sizeof(T), U = 4;
   const int ci = threadIdx.x & (cx - 1), rg = threadIdx.x / cx, groups = 256 / cx;
   const int blocks_c = (a.channels + cx * V - 1) / (cx * V);
   const unsigned tile = blockIdx.x / blocks_c;
-  const int c = ((int)(blockIdx.x - tile * blocks_c) * cx + ci) * V;
+  const int c = ((int)(blockIdx.x - tile * blocks_c) * cx + ci) * V, n = a.channels - c;
   const Rows rows = {a.d_cu_seqlens, a.d_valid, a.batch, a.t};
   const Item it = item_of(rows, tile, R * groups);
   if (it.part < 0 || it.part >= max(1, (it.len + R * groups - 1) / (R * groups))) return;
@@ -20,133 +42,137 @@ __global__ __launch_bounds__(256) void causal_conv1d_kernel(const mb_causal_conv
     slot = slot_of(a.d_slots, it.b, a.n_slots);
     if (slot < 0) return;
   }
-  if (c >= a.channels) return;
+  if (n <= 0) return;
   const T* x = (const T*)a.d_x + it.row * a.x_rstride + (a.d_cu_seqlens ? 0 : it.b * a.x_bstride) + c;
   T* y = (T*)a.d_y + it.row * a.y_rstride + (a.d_cu_seqlens ? 0 : it.b * a.y_bstride) + c;
-  float w[V][K], bias[V];
-#pragma unroll
-  for (int i = 0; i < V; ++i) {
-#pragma unroll
-    for (int j = 0; j < K; ++j) w[i][j] = a.d_w[(long long)(c + i) * K + j];
-    bias[i] = a.d_bias ? a.d_bias[c + i] : 0.f;
-  }
   const int t0 = (it.part * groups + rg) * R, t1 = min(it.len, t0 + R);
-  Vec<T, V> win[K - 1];  // rows t - K + 1 .. t - 1
   const bool first = it.part == 0 && rg == 0;
+  if (!first && t0 >= t1) return;
+  Vec<T, V> win[K - 1];  // rows t - K + 1 .. t - 1
   if (first) {
     T* st = a.d_state ? (T*)a.d_state + slot * a.state_stride + c : nullptr;
     const bool keep = st && (!a.d_has_state || a.d_has_state[it.b]);
 #pragma unroll
-    for (int j = 0; j < K - 1; ++j) {
-      if (keep) win[j] = load_vec<T, V>(st + (long long)j * a.channels);
-      else
-        for (int i = 0; i < V; ++i) win[j].v[i] = (T)0.f;
-    }
+    for (int j = 0; j < K - 1; ++j) win[j] = load_some<T, V>(st + (long long)j * a.channels, keep ? n : 0);
     if (st) {  // only this thread touches these channels of the slot: the old rows are in registers before the new ones are written
 #pragma unroll
       for (int j = 0; j < K - 1; ++j) {
         const int from = it.len + j;  // row of (state ++ x): the last K - 1 of it
         Vec<T, V> v;
-        if (from >= K - 1) v = load_vec<T, V>(x + (from - (K - 1)) * a.x_rstride);
-        else {
+        if (from >= K - 1) {
+          v = load_some<T, V>(x + (from - (K - 1)) * a.x_rstride, n);
+        } else {
 #pragma unroll
           for (int k = 0; k < K - 1; ++k)
             if (k == from) v = win[k];
         }
-        store_vec<T, V>(st + (long long)j * a.channels, v);
+        store_some<T, V>(st + (long long)j * a.channels, v, n);
       }
     }
-  } else if (t0 < t1) {  // R >= K - 1: these rows are the item's own
+    if (t0 >= t1) return;
+  } else {  // R >= K - 1: these rows are the item's own
 #pragma unroll
-    for (int j = 0; j < K - 1; ++j) win[j] = load_vec<T, V>(x + (t0 - (K - 1) + j) * a.x_rstride);
+    for (int j = 0; j < K - 1; ++j) win[j] = load_some<T, V>(x + (t0 - (K - 1) + j) * a.x_rstride, n);
   }
-  for (int t = t0; t < t1; ++t) {
-    const Vec<T, V> cur = load_vec<T, V>(x + t * a.x_rstride);
-    Vec<T, V> out;
+  float w[V][K], line[K - 1 + U][V];
+  load_taps<K, V>(a.d_w + (long long)c * K, n, w);
+  const Vec<float, V> bias = load_some<float, V>(a.d_bias + c, a.d_bias ? n : 0);
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      float v = bias[i];
+  for (int j = 0; j < K - 1; ++j)
 #pragma unroll
-      for (int j = 0; j < K - 1; ++j) v = fmaf(w[i][j], to_f32(win[j].v[i]), v);
-      v = fmaf(w[i][K - 1], to_f32(cur.v[i]), v);
-      if (a.act) v *= sigmoid<FAST>(v);
-      out.v[i] = from_f32<T>(v);
+    for (int i = 0; i < V; ++i) line[j][i] = to_f32(win[j].v[i]);
+  for (int t = t0; t < t1; t += U) {
+    Vec<T, V> cur[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) cur[u] = load_some<T, V>(x + min(t + u, t1 - 1) * a.x_rstride, n);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      Vec<T, V> out;
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        line[K - 1 + u][i] = to_f32(cur[u].v[i]);
+        float v = bias.v[i];
+#pragma unroll
+        for (int j = 0; j < K; ++j) v = fmaf(w[i][j], line[u + j][i], v);
+        if (a.act) v *= sigmoid<FAST>(v);
+        out.v[i] = from_f32<T>(v);
+      }
+      if (t + u < t1) store_some<T, V>(y + (t + u) * a.y_rstride, out, n);
     }
-    store_vec<T, V>(y + t * a.y_rstride, out);
 #pragma unroll
-    for (int j = 0; j + 1 < K - 1; ++j) win[j] = win[j + 1];
-    win[K - 2] = cur;
+    for (int j = 0; j < K - 1; ++j)
+#pragma unroll
+      for (int i = 0; i < V; ++i) line[j][i] = line[j + U][i];
   }
 }
 
 // One row per item: the same sum with the state as the window; the state moves up by one row in place.
-template <typename T, int K, int V>
+template <typename T, int K>
 __global__ __launch_bounds__(64) void causal_conv1d_step_kernel(const mb_causal_conv1d_args a) {
   constexpr bool FAST = sizeof(T) == 2;
+  constexpr int V = 8 / sizeof(T);
   const int per = (a.channels + 64 * V - 1) / (64 * V);
   const int b = (int)(blockIdx.x / per);
-  const int c = ((int)(blockIdx.x - (unsigned)b * per) * 64 + (int)threadIdx.x) * V;
+  const int c = ((int)(blockIdx.x - (unsigned)b * per) * 64 + (int)threadIdx.x) * V, n = a.channels - c;
   const int slot = slot_of(a.d_slots, b, a.n_slots);
-  if (slot < 0 || c >= a.channels) return;
-  const Vec<T, V> cur = load_vec<T, V>((const T*)a.d_x + b * a.x_rstride + c);
+  if (slot < 0 || n <= 0) return;
+  const Vec<T, V> cur = load_some<T, V>((const T*)a.d_x + b * a.x_rstride + c, n);
   T* st = (T*)a.d_state + slot * a.state_stride + c;
   Vec<T, V> win[K - 1], out;
 #pragma unroll
-  for (int j = 0; j < K - 1; ++j) win[j] = load_vec<T, V>(st + (long long)j * a.channels);
+  for (int j = 0; j < K - 1; ++j) win[j] = load_some<T, V>(st + (long long)j * a.channels, n);
+  float w[V][K];
+#pragma unroll
+  for (int i = 0; i < V; ++i)
+#pragma unroll
+    for (int j = 0; j < K; ++j) w[i][j] = i < n ? a.d_w[(long long)(c + i) * K + j] : 0.f;
+  const Vec<float, V> bias = load_some<float, V>(a.d_bias + c, a.d_bias ? n : 0);
 #pragma unroll
   for (int i = 0; i < V; ++i) {
-    const float* w = a.d_w + (long long)(c + i) * K;
-    float v = a.d_bias ? a.d_bias[c + i] : 0.f;
+    float v = bias.v[i];
 #pragma unroll
-    for (int j = 0; j < K - 1; ++j) v = fmaf(w[j], to_f32(win[j].v[i]), v);
-    v = fmaf(w[K - 1], to_f32(cur.v[i]), v);
+    for (int j = 0; j < K - 1; ++j) v = fmaf(w[i][j], to_f32(win[j].v[i]), v);
+    v = fmaf(w[i][K - 1], to_f32(cur.v[i]), v);
     if (a.act) v *= sigmoid<FAST>(v);
     out.v[i] = from_f32<T>(v);
   }
-  store_vec<T, V>((T*)a.d_y + b * a.y_rstride + c, out);
+  store_some<T, V>((T*)a.d_y + b * a.y_rstride + c, out, n);
 #pragma unroll
-  for (int j = 0; j + 1 < K - 1; ++j) store_vec<T, V>(st + (long long)j * a.channels, win[j + 1]);
-  store_vec<T, V>(st + (long long)(K - 2) * a.channels, cur);
+  for (int j = 0; j + 1 < K - 1; ++j) store_some<T, V>(st + (long long)j * a.channels, win[j + 1], n);
+  store_some<T, V>(st + (long long)(K - 2) * a.channels, cur, n);
 }
 
-template <typename T, int K, int V> int launch_conv(const mb_causal_conv1d_args& a, bool step, hipStream_t s) {
-  const int nv = (a.channels + V - 1) / V;
+template <typename T, int K> int launch_conv(const mb_causal_conv1d_args& a, bool step, hipStream_t s) {
   if (step) {
-    const long long grid = (long long)a.batch * ((nv + 63) / 64);
+    const long long grid = (long long)a.batch * cdiv(a.channels, 64 * (8 / (int)sizeof(T)));
     MB_REQUIRE(grid < (1ll << 31), "causal_conv1d_step: %d items of %d channels are too many for one launch", a.batch, a.channels);
-    hipLaunchKernelGGL((causal_conv1d_step_kernel<T, K, V>), dim3((unsigned)grid), dim3(64), 0, s, a);
+    hipLaunchKernelGGL((causal_conv1d_step_kernel<T, K>), dim3((unsigned)grid), dim3(64), 0, s, a);
   } else {
+    const int nv = cdiv(a.channels, 16 / (int)sizeof(T));
     int cx = 16;
     while (cx < 256 && cx < nv) cx *= 2;
-    const int R = 16, groups = 256 / cx;
+    // longer runs read fewer rows twice; shorter ones give every CU several workgroups
     const Rows rows = {a.d_cu_seqlens, a.d_valid, a.batch, a.t};
-    const long long grid = tiles_of(rows, R * groups) * ((nv + cx - 1) / cx);
+    int R = 32;
+    while (R > 8 && tiles_of(rows, R * (256 / cx)) * cdiv(nv, cx) < 2048) R /= 2;
+    const long long grid = tiles_of(rows, R * (256 / cx)) * cdiv(nv, cx);
     MB_REQUIRE(grid < (1ll << 31), "causal_conv1d: %d rows of %d channels are too many for one launch", a.t, a.channels);
-    hipLaunchKernelGGL((causal_conv1d_kernel<T, K, V>), dim3((unsigned)grid), dim3(256), 0, s, a, cx, R);
+    hipLaunchKernelGGL((causal_conv1d_kernel<T, K>), dim3((unsigned)grid), dim3(256), 0, s, a, cx, R);
   }
   MB_HIP(hipGetLastError());
   return MB_OK;
 }
 
-template <typename T, int V> int conv_by_taps(const mb_causal_conv1d_args& a, bool step, hipStream_t s) {
+template <typename T> int conv_by_taps(const mb_causal_conv1d_args& a, bool step, hipStream_t s) {
   switch (a.ksize) {
-    case 2: return launch_conv<T, 2, V>(a, step, s);
-    case 3: return launch_conv<T, 3, V>(a, step, s);
-    case 4: return launch_conv<T, 4, V>(a, step, s);
-    case 5: return launch_conv<T, 5, V>(a, step, s);
-    case 6: return launch_conv<T, 6, V>(a, step, s);
-    case 7: return launch_conv<T, 7, V>(a, step, s);
-    default: return launch_conv<T, 8, V>(a, step, s);
+    case 2: return launch_conv<T, 2>(a, step, s);
+    case 3: return launch_conv<T, 3>(a, step, s);
+    case 4: return launch_conv<T, 4>(a, step, s);
+    case 5: return launch_conv<T, 5>(a, step, s);
+    case 6: return launch_conv<T, 6>(a, step, s);
+    case 7: return launch_conv<T, 7>(a, step, s);
+    default: return launch_conv<T, 8>(a, step, s);
   }
-}
-
-template <typename T> int conv_by_width(const mb_causal_conv1d_args& a, bool step, hipStream_t s) {
-  constexpr int WIDE = 16 / sizeof(T);
-  // 16 bytes per access where every row of every tensor keeps that alignment; otherwise one element
-  const long long all = a.channels | a.x_rstride | a.y_rstride | (step || a.d_cu_seqlens ? 0 : a.x_bstride | a.y_bstride) |
-                        (a.d_state ? a.state_stride : 0);
-  if (all % WIDE == 0 && aligned(a.d_x, 16) && aligned(a.d_y, 16) && aligned(a.d_state, 16)) return conv_by_taps<T, WIDE>(a, step, s);
-  return conv_by_taps<T, 1>(a, step, s);
 }
 
 static int check_conv(const char* name, const mb_causal_conv1d_args* a, bool step) {
@@ -173,9 +199,9 @@ static int check_conv(const char* name, const mb_causal_conv1d_args* a, bool ste
 static int run_conv(const char* name, const mb_causal_conv1d_args* a, bool step, mb_stream_t stream) {
   const int go = check_conv(name, a, step);
   if (go <= 0) return go;
-  if (a->dtype == MB_F32) return conv_by_width<float>(*a, step, (hipStream_t)stream);
-  if (a->dtype == MB_F16) return conv_by_width<f16>(*a, step, (hipStream_t)stream);
-  return conv_by_width<bf16>(*a, step, (hipStream_t)stream);
+  if (a->dtype == MB_F32) return conv_by_taps<float>(*a, step, (hipStream_t)stream);
+  if (a->dtype == MB_F16) return conv_by_taps<f16>(*a, step, (hipStream_t)stream);
+  return conv_by_taps<bf16>(*a, step, (hipStream_t)stream);
 }
 
 }  // namespace ssm

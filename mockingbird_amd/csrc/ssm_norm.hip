@@ -19,7 +19,166 @@ __device__ __forceinline__ float block_sum(float v, float* part, int waves) {  /
   return v;
 }
 
-// Any width: one workgroup per row, three passes over the row.  Statistics are two-pass (mean, then centred squares) in fp32.
+// One pass over memory: a row (or, where the first norm's groups are all that couples channels, one group of a row) is held in
+// registers, VPT vectors of 16 bytes per thread, by one wave (WAVE: no barrier, 4 rows per workgroup) or one workgroup.  Statistics are
+// two-pass (mean, then centred squares) in fp32.  Memory-bound: 4096 channels of bf16 move 6 bytes per element for a gated norm.
+template <typename T, typename TR, int VPT, bool WAVE>
+__global__ __launch_bounds__(WAVE ? 256 : 1024) void block_norm_kernel(const mb_block_norm_args a, int parts, long long units) {
+  constexpr bool FAST = sizeof(T) == 2;
+  constexpr int V = 16 / sizeof(T);
+  __shared__ float part[16];
+  extern __shared__ float grouped[];  // groups with a next norm: a sum per vector, then mean and 1 / deviation per group
+  const int tid = WAVE ? (int)threadIdx.x & 63 : (int)threadIdx.x, width = WAVE ? 64 : (int)blockDim.x, waves = WAVE ? 1 : width / 64;
+  const long long unit = WAVE ? (long long)blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x;
+  if (WAVE && unit >= units) return;
+  const long long row = unit / parts;
+  const int C = a.channels / parts, off = (int)(unit - row * parts) * C;
+  const T* x = (const T*)a.d_x + row * a.x_rstride + off;
+  const T* gate = a.d_gate ? (const T*)a.d_gate + row * a.gate_rstride + off : nullptr;
+  const TR* res = a.d_residual ? (const TR*)a.d_residual + row * a.residual_rstride + off : nullptr;
+  const float inv_c = 1.f / C;
+  auto column = [&](int i) { return (i * width + tid) * V; };
+
+  Vec<T, V> xr[VPT], gr[VPT];
+  Vec<TR, V> rr[VPT];
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {  // everything is requested before anything is used
+    const int c = column(i), n = C - c;
+    xr[i] = load_some<T, V>(x + c, n);
+    if (gate) gr[i] = load_some<T, V>(gate + c, n);
+    if (res) rr[i] = load_some<TR, V>(res + c, n);
+  }
+  float v[VPT][V];
+#pragma unroll
+  for (int i = 0; i < VPT; ++i)
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+      v[i][k] = to_f32(xr[i].v[k]);
+      if (gate && a.gate_first) v[i][k] *= gate_of<FAST>(to_f32(gr[i].v[k]), a.gate_act);
+    }
+  // mean and 1 / deviation of the row in registers; columns beyond the row do not count
+  auto statistics = [&](int kind, float eps, float& mean, float& inv) {
+    mean = 0.f;
+    if (kind == 2) {
+#pragma unroll
+      for (int i = 0; i < VPT; ++i)
+#pragma unroll
+        for (int k = 0; k < V; ++k) mean += column(i) + k < C ? v[i][k] : 0.f;
+      mean = block_sum(mean, part, waves) * inv_c;
+    }
+    float m2 = 0.f;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i)
+#pragma unroll
+      for (int k = 0; k < V; ++k) {
+        const float d = column(i) + k < C ? v[i][k] - mean : 0.f;
+        m2 = fmaf(d, d, m2);
+      }
+    inv = 1.f / sqrtf(block_sum(m2, part, waves) * inv_c + eps);
+  };
+  auto affine = [&](const float* w, const float* b, int i) {
+    const int c = column(i), n = C - c;
+    if (w) {
+      const Vec<float, V> t = load_some<float, V>(w + off + c, n);
+#pragma unroll
+      for (int k = 0; k < V; ++k) v[i][k] *= t.v[k];
+    }
+    if (b) {
+      const Vec<float, V> t = load_some<float, V>(b + off + c, n);
+#pragma unroll
+      for (int k = 0; k < V; ++k) v[i][k] += t.v[k];
+    }
+  };
+  if (a.norm) {
+    if (WAVE || a.groups == parts) {
+      float mean, inv;
+      statistics(a.norm, a.eps, mean, inv);
+#pragma unroll
+      for (int i = 0; i < VPT; ++i)
+#pragma unroll
+        for (int k = 0; k < V; ++k) v[i][k] = (v[i][k] - mean) * inv;
+    } else {  // several groups in this row: V divides a group, every vector belongs to one
+      const int gs = C / a.groups, gv = gs / V, nv = C / V;
+      float* stat = grouped + nv;
+      for (int pass = a.norm == 2 ? 0 : 1; pass < 2; ++pass) {
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) {
+          const int c = column(i);
+          if (c >= C) continue;
+          const float mean = a.norm == 2 && pass ? stat[2 * (c / gs)] : 0.f;
+          float s = 0.f;
+#pragma unroll
+          for (int k = 0; k < V; ++k) {
+            const float d = v[i][k] - mean;
+            s = pass ? fmaf(d, d, s) : s + d;
+          }
+          grouped[c / V] = s;
+        }
+        __syncthreads();
+        for (int g = tid >> 6; g < a.groups; g += waves) {
+          float s = 0.f;
+          for (int j = tid & 63; j < gv; j += 64) s += grouped[g * gv + j];
+          s = wave_sum(s) / gs;
+          if ((tid & 63) == 0) stat[2 * g + pass] = pass ? 1.f / sqrtf(s + a.eps) : s;
+        }
+      }
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) {
+        const int c = column(i);
+        if (c >= C) continue;
+        const float mean = a.norm == 2 ? stat[2 * (c / gs)] : 0.f, inv = stat[2 * (c / gs) + 1];
+#pragma unroll
+        for (int k = 0; k < V; ++k) v[i][k] = (v[i][k] - mean) * inv;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) affine(a.d_weight, a.d_bias, i);
+  }
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    const int c = column(i), n = C - c;
+    if (gate && !a.gate_first) {
+#pragma unroll
+      for (int k = 0; k < V; ++k) v[i][k] *= gate_of<FAST>(to_f32(gr[i].v[k]), a.gate_act);
+    }
+    if (a.d_scale) {
+      const Vec<float, V> t = load_some<float, V>(a.d_scale + off + c, n);
+#pragma unroll
+      for (int k = 0; k < V; ++k) v[i][k] *= a.res_scale * t.v[k];
+    } else {
+#pragma unroll
+      for (int k = 0; k < V; ++k) v[i][k] *= a.res_scale;
+    }
+    if (res) {
+#pragma unroll
+      for (int k = 0; k < V; ++k) v[i][k] += to_f32(rr[i].v[k]);
+    }
+    if (a.d_sum) {
+      Vec<TR, V> o;
+#pragma unroll
+      for (int k = 0; k < V; ++k) o.v[k] = from_f32<TR>(v[i][k]);
+      store_some<TR, V>((TR*)a.d_sum + row * a.sum_rstride + off + c, o, n);
+    }
+  }
+  if (!a.next_norm) return;
+  float mean, inv;
+  statistics(a.next_norm, a.next_eps, mean, inv);
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    const int c = column(i), n = C - c;
+#pragma unroll
+    for (int k = 0; k < V; ++k) v[i][k] = (v[i][k] - mean) * inv;
+    affine(a.d_next_weight, a.d_next_bias, i);
+    Vec<T, V> o;
+#pragma unroll
+    for (int k = 0; k < V; ++k) o.v[k] = from_f32<T>(v[i][k]);
+    store_some<T, V>((T*)a.d_y + row * a.y_rstride + off + c, o, n);
+  }
+}
+
+// Any width, groups of any size: one workgroup per row, three passes over the row.
 template <typename T, typename TR>
 __global__ __launch_bounds__(256) void block_norm_row_kernel(const mb_block_norm_args a) {
   constexpr bool FAST = sizeof(T) == 2;
@@ -88,7 +247,31 @@ __global__ __launch_bounds__(256) void block_norm_row_kernel(const mb_block_norm
 }
 
 template <typename T, typename TR> int launch_norm(const mb_block_norm_args& a, hipStream_t s) {
-  hipLaunchKernelGGL((block_norm_row_kernel<T, TR>), dim3((unsigned)a.rows), dim3(256), (size_t)2 * a.groups * sizeof(float), s, a);
+  constexpr int V = 16 / sizeof(T);
+  // groups couple nothing but themselves without a next norm: each is a row of its own
+  const int parts = a.next_norm ? 1 : a.groups, C = a.channels / parts, nv = cdiv(C, V);
+  const long long units = a.rows * parts;
+  const bool grouped = a.groups != parts;
+  // One wave per row up to 256 vectors; with few rows a wider row is dealt to a workgroup, whose loads are then in flight at once.
+  const bool wave = !grouped && nv <= 256 && (nv <= 64 || units >= 1024);
+  const bool whole = nv <= 4096 && (!grouped || (C / a.groups) % V == 0) && units < (1ll << 31);
+  const size_t lds = whole && !wave && grouped ? ((size_t)nv + 2 * a.groups) * sizeof(float) : 0;
+#define MB_NORM(VPT, WAVE, GRID, THREADS) \
+  hipLaunchKernelGGL((block_norm_kernel<T, TR, VPT, WAVE>), dim3((unsigned)(GRID)), dim3(THREADS), lds, s, a, parts, units)
+  if (whole && wave) {
+    const long long grid = (units + 3) / 4;
+    if (nv <= 64) MB_NORM(1, true, grid, 256);
+    else if (nv <= 128) MB_NORM(2, true, grid, 256);
+    else MB_NORM(4, true, grid, 256);
+  } else if (whole) {
+    const int vpt = nv <= 512 ? 1 : nv <= 2048 ? 2 : 4, threads = (cdiv(nv, vpt) + 63) / 64 * 64;
+    if (vpt == 1) MB_NORM(1, false, units, threads);
+    else if (vpt == 2) MB_NORM(2, false, units, threads);
+    else MB_NORM(4, false, units, threads);
+  } else {
+    hipLaunchKernelGGL((block_norm_row_kernel<T, TR>), dim3((unsigned)a.rows), dim3(256), (size_t)2 * a.groups * sizeof(float), s, a);
+  }
+#undef MB_NORM
   MB_HIP(hipGetLastError());
   return MB_OK;
 }

@@ -4,41 +4,17 @@
 namespace mb {
 namespace ssm {
 
-// Four state columns n .. n+3 of a row; columns from `left` on do not exist and stay zero.  VEC: rows of whole, 16-byte aligned quads.
-template <bool VEC> __device__ __forceinline__ f32x4 load_quad(const float* p, int left) {
-  if (VEC) return left > 0 ? *(const f32x4*)p : f32x4{0.f, 0.f, 0.f, 0.f};
-  f32x4 v = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (i < left) v[i] = p[i];
-  return v;
-}
-template <bool VEC> __device__ __forceinline__ void store_quad(float* p, f32x4 v, int left) {
-  if (VEC) {
-    if (left > 0) *(f32x4*)p = v;
-    return;
-  }
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (i < left) p[i] = v[i];
-}
-template <typename T> __device__ __forceinline__ f32x4 load_quad_of(const T* p, int left) {
-  f32x4 v = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (i < left) v[i] = to_f32(p[i]);
-  return v;
-}
 template <int LANES> __device__ __forceinline__ float lanes_sum(float v) {
 #pragma unroll
   for (int o = LANES / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
   return v;
 }
 
-// One row per item.  LANES lanes hold a state row (4 columns each), 256 / LANES rows at a time; a workgroup takes `pb` rows of one head.
-template <typename T, int LANES, bool VEC>
+// One row per item: the state is read and written once (8 bytes per element of it), which is all that counts with many items.  LANES
+// lanes hold a state row (4 columns each), 256 / LANES rows at a time; a workgroup takes `pb` rows of one head, U passes requested at once.
+template <typename T, int LANES>
 __global__ __launch_bounds__(256) void selective_scan_step_kernel(const mb_selective_scan_args a, int pb) {
-  constexpr int ROWS = 256 / LANES;
+  constexpr int ROWS = 256 / LANES, U = 4;
   const int splits = (a.head_dim + pb - 1) / pb;
   const unsigned item_head = blockIdx.x / splits;
   const int p0 = (int)(blockIdx.x - item_head * splits) * pb;
@@ -47,27 +23,45 @@ __global__ __launch_bounds__(256) void selective_scan_step_kernel(const mb_selec
   if (slot < 0) return;
   const int n = (int)(threadIdx.x % LANES) * 4, left = a.d_state_dim - n;
   const int group = head / (a.heads / a.groups);
-  const float d = step_size(a, b * a.dt_rstride + head, head);
-  const float decay = expf(d * a.d_a[head]), skip = a.d_d ? a.d_d[head] : 0.f;
-  const f32x4 bv = load_quad_of((const T*)a.d_b + b * a.b_rstride + (long long)group * a.d_state_dim + n, left);
-  const f32x4 cv = load_quad_of((const T*)a.d_c + b * a.c_rstride + (long long)group * a.d_state_dim + n, left);
+  const int p1 = min(a.head_dim, p0 + pb);
+  float* h = a.d_state + slot * a.state_stride + (long long)head * a.head_dim * a.d_state_dim + n;
   const T* x = (const T*)a.d_x + b * a.x_rstride + (long long)head * a.head_dim;
   T* y = (T*)a.d_y + b * a.y_rstride + (long long)head * a.head_dim;
-  float* h = a.d_state + slot * a.state_stride + (long long)head * a.head_dim * a.d_state_dim + n;
-  const int p1 = min(a.head_dim, p0 + pb);
-#pragma unroll 4
-  for (int p = p0 + (int)threadIdx.x / LANES; p < p1; p += ROWS) {
-    f32x4 v = load_quad<VEC>(h + (long long)p * a.d_state_dim, left);
-    const float xv = to_f32(x[p]), dx = d * xv;
-    float s = 0.f;
+  float decay = 0.f, d = 0.f;
+  Vec<T, 4> br, cr;
+  const float skip = a.d_d ? a.d_d[head] : 0.f;
+  for (int q = p0; q < p1; q += U * ROWS) {
+    const int p = q + (int)threadIdx.x / LANES;
+    Vec<float, 4> v[U];
+    float xv[U];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      v[i] = fmaf(v[i], decay, dx * bv[i]);
-      s = fmaf(v[i], cv[i], s);
+    for (int u = 0; u < U; ++u) {
+      const int r = p + u * ROWS;
+      v[u] = load_some<float, 4>(h + (long long)r * a.d_state_dim, r < p1 ? left : 0);
+      xv[u] = r < p1 ? to_f32(x[r]) : 0.f;
     }
-    store_quad<VEC>(h + (long long)p * a.d_state_dim, v, left);
-    s = lanes_sum<LANES>(s);
-    if (n == 0) y[p] = from_f32<T>(fmaf(skip, xv, s));
+    if (q == p0) {  // behind the first states' requests
+      br = load_some<T, 4>((const T*)a.d_b + b * a.b_rstride + (long long)group * a.d_state_dim + n, left);
+      cr = load_some<T, 4>((const T*)a.d_c + b * a.c_rstride + (long long)group * a.d_state_dim + n, left);
+      d = step_size(a, b * a.dt_rstride + head, head);
+      decay = expf(d * a.d_a[head]);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int r = p + u * ROWS;
+      const float dx = d * xv[u];
+      float s = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        v[u].v[i] = fmaf(v[u].v[i], decay, dx * to_f32(br.v[i]));
+        s = fmaf(v[u].v[i], to_f32(cr.v[i]), s);
+      }
+      s = lanes_sum<LANES>(s);
+      if (r < p1) {
+        store_some<float, 4>(h + (long long)r * a.d_state_dim, v[u], left);
+        if (n == 0) y[r] = from_f32<T>(fmaf(skip, xv[u], s));
+      }
+    }
   }
 }
 
@@ -110,29 +104,24 @@ __global__ __launch_bounds__(256) void selective_scan_join_kernel(const mb_selec
   }
 }
 
-template <typename T, int LANES, bool VEC> int launch_step(const mb_selective_scan_args& a, hipStream_t s) {
+template <typename T, int LANES> int launch_step(const mb_selective_scan_args& a, hipStream_t s) {
   constexpr int ROWS = 256 / LANES;
   int pb = (a.head_dim + ROWS - 1) / ROWS * ROWS;
   // few requests: a head's rows are dealt to more workgroups, down to one pass each, until two fit every CU
   while (pb > ROWS && (long long)a.batch * a.heads * ((a.head_dim + pb - 1) / pb) < 512) pb = (pb / ROWS + 1) / 2 * ROWS;
   const long long grid = (long long)a.batch * a.heads * ((a.head_dim + pb - 1) / pb);
   MB_REQUIRE(grid < (1ll << 31), "selective_scan_step: %d items of %d heads are too many for one launch", a.batch, a.heads);
-  hipLaunchKernelGGL((selective_scan_step_kernel<T, LANES, VEC>), dim3((unsigned)grid), dim3(256), 0, s, a, pb);
+  hipLaunchKernelGGL((selective_scan_step_kernel<T, LANES>), dim3((unsigned)grid), dim3(256), 0, s, a, pb);
   MB_HIP(hipGetLastError());
   return MB_OK;
 }
 
-template <typename T, bool VEC> int step_by_lanes(const mb_selective_scan_args& a, hipStream_t s) {
-  if (a.d_state_dim <= 16) return launch_step<T, 4, VEC>(a, s);
-  if (a.d_state_dim <= 32) return launch_step<T, 8, VEC>(a, s);
-  if (a.d_state_dim <= 64) return launch_step<T, 16, VEC>(a, s);
-  if (a.d_state_dim <= 128) return launch_step<T, 32, VEC>(a, s);
-  return launch_step<T, 64, VEC>(a, s);
-}
-
-template <typename T> int step_by_width(const mb_selective_scan_args& a, hipStream_t s) {
-  const bool vec = a.d_state_dim % 4 == 0 && aligned(a.d_state, 16) && a.state_stride % 4 == 0;
-  return vec ? step_by_lanes<T, true>(a, s) : step_by_lanes<T, false>(a, s);
+template <typename T> int step_by_lanes(const mb_selective_scan_args& a, hipStream_t s) {
+  if (a.d_state_dim <= 16) return launch_step<T, 4>(a, s);
+  if (a.d_state_dim <= 32) return launch_step<T, 8>(a, s);
+  if (a.d_state_dim <= 64) return launch_step<T, 16>(a, s);
+  if (a.d_state_dim <= 128) return launch_step<T, 32>(a, s);
+  return launch_step<T, 64>(a, s);
 }
 
 // Rows of a time tile, or 0 for one workgroup walking a whole item.  A tile's workgroups carry units_of() heads' states; about 512
@@ -208,7 +197,7 @@ static int run_scan(const mb_selective_scan_args* a, void* ws, size_t ws_bytes, 
 static int run_step(const mb_selective_scan_args* a, hipStream_t s) {
   const int go = check_scan("selective_scan_step", a, true);
   if (go <= 0) return go;
-  return a->dtype == MB_F32 ? step_by_width<float>(*a, s) : a->dtype == MB_F16 ? step_by_width<f16>(*a, s) : step_by_width<bf16>(*a, s);
+  return a->dtype == MB_F32 ? step_by_lanes<float>(*a, s) : a->dtype == MB_F16 ? step_by_lanes<f16>(*a, s) : step_by_lanes<bf16>(*a, s);
 }
 
 }  // namespace ssm

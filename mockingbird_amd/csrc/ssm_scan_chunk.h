@@ -136,15 +136,14 @@ template <int STRIDE> __device__ __forceinline__ bf16x8 read_row(const unsigned 
 template <typename T, int V, int ROWS, int COLS, int THREADS> struct Stage {
   static constexpr int PER_ROW = COLS / V, TOTAL = ROWS * PER_ROW, COUNT = (TOTAL + THREADS - 1) / THREADS;
   Vec<T, V> v[COUNT];
-  // col(c) -> offset of column c from the row, or -1 where the tensor has none; rows from `rows` on are zero
+  // col(c, n) -> offset of column c from the row, n = how many columns the tensor has from there on; rows from `rows` on are zero
   template <typename F> __device__ __forceinline__ void request(const T* base, long long rstride, int rows, F col) {
 #pragma unroll
     for (int i = 0; i < COUNT; ++i) {
       const int at = (int)threadIdx.x + i * THREADS, r = at / PER_ROW, c = at % PER_ROW * V;
-#pragma unroll
-      for (int k = 0; k < V; ++k) v[i].v[k] = (T)0.f;
-      const int off = col(c);
-      if (r < rows && off >= 0) v[i] = load_vec<T, V>(base + r * rstride + off);
+      int n = 0;
+      const int off = col(c, n);
+      v[i] = load_some<T, V>(base + r * rstride + off, r < rows ? n : 0);
     }
   }
   // put(plane, row, column, V halves)
@@ -184,10 +183,10 @@ struct Split {
 };
 
 // STATES: first pass of a split call, the state every tile adds to a zero state.  Otherwise y (and the final states).
-template <typename T, int NP, int V, bool STATES>
+template <typename T, int NP, bool STATES>
 __global__ __launch_bounds__((ScanShape<T, NP>::THREADS)) void selective_scan_chunk_kernel(const mb_selective_scan_args a, const Split sp) {
   typedef ScanShape<T, NP> S;
-  constexpr int R = S::R, Q = S::Q, L = S::L, HB = S::HB, TT = S::TT, NT = S::NT, PB = S::PB, THREADS = S::THREADS;
+  constexpr int V = 16 / sizeof(T), R = S::R, Q = S::Q, L = S::L, HB = S::HB, TT = S::TT, NT = S::NT, PB = S::PB, THREADS = S::THREADS;
   extern __shared__ __attribute__((aligned(16))) char lds_raw[];
   typename S::Lds& m = *(typename S::Lds*)lds_raw;
 
@@ -230,23 +229,13 @@ __global__ __launch_bounds__((ScanShape<T, NP>::THREADS)) void selective_scan_ch
   if (a.d_state && !sp.seg) st = a.d_state + slot * a.state_stride + head * head_state;
   const float* from = sp.seg ? sp.state + ((long long)tile * a.heads + head) * head_state : st;
   const bool keep = !STATES && (sp.seg ? true : st && (!a.d_has_state || a.d_has_state[it.b]));
-  const bool quads = a.d_state_dim % 4 == 0 && (sp.seg || (aligned(a.d_state, 16) && a.state_stride % 4 == 0));
 #pragma unroll
   for (int pt = 0; pt < 2; ++pt)
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const int p = p0 + pw + 16 * pt + li, n = 16 * nt + 4 * g;
-      h[pt][nt] = f32x4{0.f, 0.f, 0.f, 0.f};
-      if (keep && mine && p < a.head_dim) {
-        const float* src = from + (long long)p * a.d_state_dim + n;
-        if (quads) {
-          if (n < a.d_state_dim) h[pt][nt] = *(const f32x4*)src;
-        } else {
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (n + i < a.d_state_dim) h[pt][nt][i] = src[i];
-        }
-      }
+      const int left = keep && mine && p < a.head_dim ? a.d_state_dim - n : 0;
+      h[pt][nt] = __builtin_bit_cast(f32x4, load_some<float, 4>(from + (long long)p * a.d_state_dim + n, left));
     }
 
   Stage<T, V, L, NP, THREADS> sb, sc;
@@ -254,12 +243,16 @@ __global__ __launch_bounds__((ScanShape<T, NP>::THREADS)) void selective_scan_ch
   float draw = 0.f;
   auto request = [&](int t) {
     const int n = t1 - t;
-    auto col_n = [&](int c) { return c < a.d_state_dim ? c : -1; };
+    auto col_n = [&](int c, int& left) {
+      left = a.d_state_dim - c;
+      return c;
+    };
     sb.request(bg + t * a.b_rstride, a.b_rstride, n, col_n);
     if (!STATES) sc.request(cg + t * a.c_rstride, a.c_rstride, n, col_n);
-    sx.request(xg + t * a.x_rstride, a.x_rstride, n, [&](int c) {
+    sx.request(xg + t * a.x_rstride, a.x_rstride, n, [&](int c, int& left) {
       const int i = c / PB, p = c % PB;
-      return i < live && p0 + p < a.head_dim ? i * a.head_dim + p : -1;
+      left = i < live ? a.head_dim - p0 - p : 0;
+      return i * a.head_dim + p;
     });
     if (half == 0 && mine && lane < L && lane < n) draw = step_raw(a, dtg + (t + lane) * a.dt_rstride + head);
   };
@@ -479,18 +472,10 @@ __global__ __launch_bounds__((ScanShape<T, NP>::THREADS)) void selective_scan_ch
             const int p = p0 + pw + 16 * pt + 4 * g;
             if (row < t1) {
               T* dst = yg + row * a.y_rstride + (long long)hh * a.head_dim + pw + 16 * pt + 4 * g;
-              if (V > 1) {
-                if (p < a.head_dim) {
-                  Vec<T, 4> o;
+              Vec<T, 4> o;
 #pragma unroll
-                  for (int r = 0; r < 4; ++r) o.v[r] = from_f32<T>(acc[j][pt][r]);
-                  store_vec<T, 4>(dst, o);
-                }
-              } else {
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-                  if (p + r < a.head_dim) dst[r] = from_f32<T>(acc[j][pt][r]);
-              }
+              for (int r = 0; r < 4; ++r) o.v[r] = from_f32<T>(acc[j][pt][r]);
+              store_some<T, 4>(dst, o, a.head_dim - p);
             }
           }
         }
@@ -506,25 +491,16 @@ __global__ __launch_bounds__((ScanShape<T, NP>::THREADS)) void selective_scan_ch
   }
   if (!mine) return;
   float* to = STATES ? sp.state + ((long long)tile * a.heads + head) * head_state : a.d_state + slot * a.state_stride + head * head_state;
-  const bool whole = a.d_state_dim % 4 == 0 && (STATES || (aligned(a.d_state, 16) && a.state_stride % 4 == 0));
 #pragma unroll
   for (int pt = 0; pt < 2; ++pt)
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const int p = p0 + pw + 16 * pt + li, n = 16 * nt + 4 * g;
-      if (p >= a.head_dim) continue;
-      float* dst = to + (long long)p * a.d_state_dim + n;
-      if (whole) {
-        if (n < a.d_state_dim) *(f32x4*)dst = h[pt][nt];
-      } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (n + i < a.d_state_dim) dst[i] = h[pt][nt][i];
-      }
+      if (p < a.head_dim) store_some<float, 4>(to + (long long)p * a.d_state_dim + n, __builtin_bit_cast(Vec<float, 4>, h[pt][nt]), a.d_state_dim - n);
     }
 }
 
-template <typename T, int NP, int V, bool STATES> int launch_chunk(const mb_selective_scan_args& a, const Split& sp, hipStream_t s) {
+template <typename T, int NP, bool STATES> int launch_chunk(const mb_selective_scan_args& a, const Split& sp, hipStream_t s) {
   typedef ScanShape<T, NP> S;
   static_assert(sizeof(typename S::Lds) <= 160 * 1024, "a chunk has to fit LDS");
   static std::atomic<unsigned long long> attr_done{0};  // per device: the attribute belongs to the function on the current device
@@ -532,7 +508,7 @@ template <typename T, int NP, int V, bool STATES> int launch_chunk(const mb_sele
   MB_HIP(hipGetDevice(&dev));
   const unsigned long long bit = dev >= 0 && dev < 64 ? 1ull << dev : 0ull;
   if (!bit || !(attr_done.load(std::memory_order_acquire) & bit)) {
-    MB_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(&selective_scan_chunk_kernel<T, NP, V, STATES>),
+    MB_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(&selective_scan_chunk_kernel<T, NP, STATES>),
                                hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
     attr_done.fetch_or(bit, std::memory_order_release);
   }
@@ -541,26 +517,15 @@ template <typename T, int NP, int V, bool STATES> int launch_chunk(const mb_sele
   const long long units = (long long)a.groups * cdiv(per_group, S::HB) * cdiv(a.head_dim, S::PB);
   const long long grid = tiles_of(rows, sp.seg ? sp.seg : (a.t > 1 ? a.t : 1)) * units;
   MB_REQUIRE(grid < (1ll << 31), "selective_scan: %d items of %d heads are too many for one launch", a.batch, a.heads);
-  hipLaunchKernelGGL((selective_scan_chunk_kernel<T, NP, V, STATES>), dim3((unsigned)grid), dim3(S::THREADS), sizeof(typename S::Lds), s, a, sp);
+  hipLaunchKernelGGL((selective_scan_chunk_kernel<T, NP, STATES>), dim3((unsigned)grid), dim3(S::THREADS), sizeof(typename S::Lds), s, a, sp);
   MB_HIP(hipGetLastError());
   return MB_OK;
 }
 
-template <typename T, int V> int chunk_by_width(const mb_selective_scan_args& a, const Split& sp, bool states, hipStream_t s) {
-  if (a.d_state_dim <= 64) return states ? launch_chunk<T, 64, V, true>(a, sp, s) : launch_chunk<T, 64, V, false>(a, sp, s);
-  if (a.d_state_dim <= 128) return states ? launch_chunk<T, 128, V, true>(a, sp, s) : launch_chunk<T, 128, V, false>(a, sp, s);
-  return states ? launch_chunk<T, 256, V, true>(a, sp, s) : launch_chunk<T, 256, V, false>(a, sp, s);
-}
-
-// 16 bytes per access where head_dim, d_state and every row keep that alignment (y: 4 elements), one element otherwise
 template <typename T> int chunk_launch(const mb_selective_scan_args& a, const Split& sp, bool states, hipStream_t s) {
-  constexpr int WIDE = 16 / sizeof(T);
-  const bool padded = !a.d_cu_seqlens;
-  const long long all = a.head_dim | a.d_state_dim | a.x_rstride | a.b_rstride | a.c_rstride | a.y_rstride |
-                        (padded ? a.x_bstride | a.b_bstride | a.c_bstride | a.y_bstride : 0);
-  if (all % WIDE == 0 && aligned(a.d_x, 16) && aligned(a.d_b, 16) && aligned(a.d_c, 16) && aligned(a.d_y, 16))
-    return chunk_by_width<T, WIDE>(a, sp, states, s);
-  return chunk_by_width<T, 1>(a, sp, states, s);
+  if (a.d_state_dim <= 64) return states ? launch_chunk<T, 64, true>(a, sp, s) : launch_chunk<T, 64, false>(a, sp, s);
+  if (a.d_state_dim <= 128) return states ? launch_chunk<T, 128, true>(a, sp, s) : launch_chunk<T, 128, false>(a, sp, s);
+  return states ? launch_chunk<T, 256, true>(a, sp, s) : launch_chunk<T, 256, false>(a, sp, s);
 }
 
 // the kernels of one type each, in ssm_scan_{f32,f16,bf16}.hip
