@@ -65,18 +65,20 @@ __global__ __launch_bounds__(256) void selective_scan_step_kernel(const mb_selec
   }
 }
 
-// Between the two passes of a split call: every tile's own sum becomes the state in front of it.
+// Between the two passes of a split call: every tile's own sum becomes the state in front of it.  4 elements per thread; the tiles are
+// read U ahead of the chain that runs over them.
 __global__ __launch_bounds__(256) void selective_scan_join_kernel(const mb_selective_scan_args a, const Split sp) {
-  const int elems = a.head_dim * a.d_state_dim, blocks = (elems + 255) / 256;
+  constexpr int U = 4;
+  const int elems = a.head_dim * a.d_state_dim, blocks = (elems + 1023) / 1024;
   const unsigned item_head = blockIdx.x / blocks;
-  const int e = (int)(blockIdx.x - item_head * blocks) * 256 + (int)threadIdx.x;
+  const int e = ((int)(blockIdx.x - item_head * blocks) * 256 + (int)threadIdx.x) * 4, n = elems - e;
   const int b = (int)(item_head / a.heads), head = (int)(item_head - (unsigned)b * a.heads);
   int slot = -1;
   if (a.d_state) {
     slot = slot_of(a.d_slots, b, a.n_slots);
     if (slot < 0) return;
   }
-  if (e >= elems) return;
+  if (n <= 0) return;
   long long tile;
   int len;
   if (a.d_cu_seqlens) {
@@ -88,19 +90,27 @@ __global__ __launch_bounds__(256) void selective_scan_join_kernel(const mb_selec
     tile = (long long)b * (a.t > sp.seg ? (a.t + sp.seg - 1) / sp.seg : 1);
   }
   const int parts = max(1, (len + sp.seg - 1) / sp.seg);
-  float h = 0.f;
-  if (a.d_state && (!a.d_has_state || a.d_has_state[b])) h = a.d_state[slot * a.state_stride + (long long)head * elems + e];
+  const bool keep = a.d_state && (!a.d_has_state || a.d_has_state[b]);
+  Vec<float, 4> h = load_some<float, 4>(a.d_state + slot * a.state_stride + (long long)head * elems + e, keep ? n : 0);
   const long long step = (long long)a.heads * elems;
   float* st = sp.state + (tile * a.heads + head) * (long long)elems + e;
   const float* decay = sp.decay + tile * a.heads + head;
-  float own = 0.f, next = parts > 1 ? st[0] : 0.f;
-  for (int k = 0; k < parts; ++k) {
-    own = next;
-    if (k + 2 < parts) next = st[step];  // the last tile's own sum is not computed: nothing follows it
-    st[0] = h;
-    if (k + 1 < parts) h = fmaf(h, *decay, own);
-    st += step;
-    decay += a.heads;
+  for (int k = 0; k < parts; k += U) {
+    Vec<float, 4> own[U];
+    float by[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {  // the last tile's own sum is not computed: nothing follows it
+      own[u] = load_some<float, 4>(st + u * step, k + u + 1 < parts ? n : 0);
+      by[u] = k + u + 1 < parts ? decay[(long long)u * a.heads] : 0.f;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (k + u < parts) store_some<float, 4>(st + u * step, h, n);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) h.v[i] = fmaf(h.v[i], by[u], own[u].v[i]);
+    }
+    st += U * step;
+    decay += (long long)U * a.heads;
   }
 }
 
@@ -124,11 +134,10 @@ template <typename T> int step_by_lanes(const mb_selective_scan_args& a, hipStre
   return launch_step<T, 64>(a, s);
 }
 
-// Rows of a time tile, or 0 for one workgroup walking a whole item.  A tile's workgroups carry units_of() heads' states; about 512
-// workgroups (two per CU) are wanted.  The host does not know the lengths of packed items: it deals out the rows of all together.
+// Rows of a time tile, or 0 for one workgroup walking a whole item.  About 512 workgroups (two per CU) are wanted.  The host does not
+// know the lengths of packed items: it deals out the rows of all together.
 static int rows_per_tile(const mb_selective_scan_args& a) {
-  const int hb = a.dtype == MB_F32 && a.d_state_dim > 128 ? 2 : 4;
-  const long long units = (long long)a.groups * cdiv(a.heads / a.groups, hb) * cdiv(a.head_dim, 64);
+  const long long units = (long long)a.groups * cdiv(a.heads / a.groups, 2) * cdiv(a.head_dim, 64);
   const long long all = a.d_cu_seqlens ? a.t : (long long)a.t * a.batch;
   long long seg = (all * units + 511) / 512;
   if (seg < 256) seg = 256;
@@ -186,7 +195,7 @@ static int run_scan(const mb_selective_scan_args* a, void* ws, size_t ws_bytes, 
   if (sp.seg) {
     const int rc = chunks(*a, sp, true, s);
     if (rc) return rc;
-    const long long grid = (long long)a->batch * a->heads * cdiv(a->head_dim * a->d_state_dim, 256);
+    const long long grid = (long long)a->batch * a->heads * cdiv(a->head_dim * a->d_state_dim, 1024);
     MB_REQUIRE(grid < (1ll << 31), "selective_scan: %d items of %d heads are too many for one launch", a->batch, a->heads);
     hipLaunchKernelGGL(selective_scan_join_kernel, dim3((unsigned)grid), dim3(256), 0, s, *a, sp);
     MB_HIP(hipGetLastError());

@@ -3,12 +3,17 @@
 //   h   <- exp(s(L)) h + sum_s exp(s(L) - s(s)) d_s x_s B_s^T
 // i.e. four products per chunk and head: G = C B^T (shared by the heads of a group), M x, C h, and x^T B.
 //
-// A workgroup takes HB heads of one group and 64 of their columns (two waves per head, 32 columns each) and walks along time; h stays
+// A workgroup takes two heads of one group and 64 of their columns (two waves per head, 32 columns each) and walks along time; h stays
 // in the accumulators (fp32) of those waves for the whole walk and never visits LDS or memory between chunks.  Every product is written
-// so that one factor is already in the register layout the matrix instruction wants: the accumulator layout of 16x16x32 products (column = lane
-// & 15, rows 4 (lane >> 4) + i) of two stacked tiles IS an operand whose inner index runs 4 g + i, 16 + 4 g + i, so G^T feeds M x and
-// h feeds C h directly, provided the other operand is read in the same order -- C as two 8-byte LDS reads, x^T and B^T as two
-// transposing reads.
+// so that one factor is already in the register layout the matrix instruction wants: in the accumulators of two stacked 16x16x32 tiles a
+// lane holds rows 4 g + i of both (g = lane >> 4) of column lane & 15, which is an operand whose inner index is dealt out as those rows.
+// So G^T tiles become M^T operands and h tiles operands of C h without moving between lanes, provided the other operand is read in the same
+// order: x^T by transposing reads of rows 4 g + i and 16 + 4 g + i; for C h the state's rows are numbered so that the order is C's own
+// (tile 2 q holds columns 32 q + 8 g + i, tile 2 q + 1 those 4 further on).
+//
+// Two workgroups fit a CU: while one waits at a barrier or converts operands, the other's products run.  What bounds it is the vector
+// pipe (splitting h, M and c x into planes), not the matrix pipe; hence M is formed once per head and goes through LDS, and B, C are
+// shared by two heads only.
 //
 // Precision.  Every sum, the state and all exponents are fp32 (prefix sums over a chunk: fp64, so that differences of far rows keep
 // their bits).  Operands are bf16 planes: a raw value is exact in 1 (bf16), 2 (fp16) or 3 (fp32) planes; computed operands are split as
@@ -70,10 +75,11 @@ __device__ __forceinline__ float value_of(const bf16x8& v, int i) {
 // a NaN or infinity among 8 values
 __device__ __forceinline__ bool not_finite(const bf16x8& v) {
   const u32x4 w = __builtin_bit_cast(u32x4, v);
-  bool any = false;
+  typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+  u16x2 top = {0, 0};
 #pragma unroll
-  for (int i = 0; i < 4; ++i) any |= (w[i] & 0x7f80u) == 0x7f80u || (w[i] & 0x7f800000u) == 0x7f800000u;
-  return any;
+  for (int i = 0; i < 4; ++i) top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, w[i] & 0x7fff7fffu));
+  return top[0] >= 0x7f80 || top[1] >= 0x7f80;
 }
 
 // acc += a b over the plane pairs whose product is above 2^-8(K): K planes of the result are kept
@@ -90,21 +96,26 @@ __device__ __forceinline__ f32x4 mma(const bf16x8 (&a)[QA], const bf16x8 (&b)[QB
 template <typename T, int NP> struct ScanShape {
   static constexpr int R = sizeof(T) == 4 ? 3 : std::is_same<T, f16>::value ? 2 : 1;  // raw planes
   static constexpr int Q = R == 3 ? 3 : 2;                                             // planes of M and h
-  static constexpr int L = R == 1 && NP <= 128 ? 64 : 32;  // rows of a chunk: 64 where LDS and registers hold them
-  static constexpr int HB = R == 3 && NP == 256 ? 2 : 4;   // heads of a workgroup
+  static constexpr int L = R == 1 && NP <= 128 ? 64 : 32;  // rows of a chunk: 64 where two workgroups' LDS and registers hold them
+  static constexpr int HB = 2;                             // heads of a workgroup
   static constexpr int PB = 64;                            // columns of a workgroup
-  static constexpr int THREADS = HB * 128;
+  static constexpr int PT = 1;                             // 16-column tiles of a wave
+  static constexpr int WPH = PB / (16 * PT);               // waves per head
+  static constexpr int THREADS = HB * WPH * 64;
   static constexpr int TT = L / 16;                        // row tiles
   static constexpr int NT = NP / 16;                       // state tiles
-  // LDS rows are 32 bytes longer than their data: 16 rows of 32 bytes (a wave's 8-byte and transposing reads) meet every bank twice
-  static constexpr int NS = NP + 16, XS = PB + 16;         // row strides in halves
+  // LDS rows of B and C are 32 bytes longer than their data: 8 rows of one 16-byte unit lie in different banks.  x has no room for that (two
+  // workgroups would not fit): its 32-byte pieces change places with the row, so that 4 rows of one piece do.
+  static constexpr int NS = NP + 16;                       // row stride in halves
+  static __device__ __forceinline__ int x_col(int r, int c) { return c ^ 16 * (r >> 1 & 1); }
   static constexpr int GT = TT * (TT + 1) / 2;             // causal tiles of G
-  struct alignas(16) Head { float u[L], w[L], pre[L], cs[L], hi[L], lo[L], d[L], f[TT][TT], total; };
+  struct alignas(16) Head { float u[L], w[L], hi[L], lo[L], d[L], f[TT][TT], front[TT], back[TT], total; };
   struct Lds {
-    unsigned short b[R][L][NS], c[R][L][NS], x[HB][R][L][XS];
-    f32x4 g[GT][64];
-    Head head[HB];
+    unsigned short b[R][L][NS], c[R][L][NS], x[HB][R][L][PB];
+    bf16x4 m[HB][GT][Q][64];
+    Head head[2][HB];  // of this chunk and the next
   };
+  static constexpr int WAVES = (sizeof(Lds) <= 80 * 1024 ? 2 : 1) * THREADS / 256;  // per SIMD, of the workgroups that share a CU
 };
 
 // Waves of a workgroup meet; LDS written before is visible behind it.  Loads from global memory stay in flight.
@@ -114,22 +125,18 @@ __device__ __forceinline__ void meet() {
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
-// 8 rows t (or s) of one column as an operand: rows t0 + 4 g + i and t0 + 16 + 4 g + i, column c0 + (lane & 15) of a row-major tile.
-// Each group of 16 lanes hands in the 16 quads of its 4 rows and gets them back transposed.
-template <int STRIDE> __device__ __forceinline__ bf16x8 read_transposed(const unsigned short (*m)[STRIDE], int t0, int c0, int lane) {
+// 8 rows of one column as an operand, out of LDS: each group of 16 lanes hands in the quads (4 columns) of its 4 rows and gets the 16
+// columns back transposed.  lo: this lane's quad in rows 4 g + i, hi: in rows 16 + 4 g + i.
+__device__ __forceinline__ bf16x8 read_transposed(const unsigned short* lo, const unsigned short* hi) {
   typedef __attribute__((address_space(3))) s16x4 lds4;
-  const int g = lane >> 4, i = lane & 15;
-  const unsigned short* p = &m[t0 + 4 * g + (i >> 2)][c0 + 4 * (i & 3)];
-  const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)p);
-  const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(p + 16 * STRIDE));
   typedef short s16x8 __attribute__((ext_vector_type(8)));
-  const s16x8 v = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+  const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)lo), b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)hi);
+  const s16x8 v = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
   return __builtin_bit_cast(bf16x8, v);
 }
-// Row r of a row-major tile: columns c0 + 4 g + i and c0 + 16 + 4 g + i.
-template <int STRIDE> __device__ __forceinline__ bf16x8 read_row(const unsigned short (*m)[STRIDE], int r, int c0, int g) {
-  const bf16x4 lo = *(const bf16x4*)&m[r][c0 + 4 * g], hi = *(const bf16x4*)&m[r][c0 + 16 + 4 * g];
-  return bf16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+template <int V> __device__ __forceinline__ void store_lds(unsigned short* p, const Vec<unsigned short, V>& v) {
+  typedef unsigned short vt __attribute__((ext_vector_type(V)));
+  *(vt*)p = __builtin_bit_cast(vt, v);  // aligned: rows of 16-byte multiples, columns of V
 }
 
 // Raw values on their way to LDS: COUNT vectors of V per thread, requested a chunk ahead.  COLS (a power of two) values per row.
@@ -146,11 +153,22 @@ template <typename T, int V, int ROWS, int COLS, int THREADS> struct Stage {
       v[i] = load_some<T, V>(base + r * rstride + off, r < rows ? n : 0);
     }
   }
+  // The same where every column exists: through a buffer descriptor that ends behind row `rows` - 1, whose range check supplies the zeros.
+  // One address register for all; the thread's further vectors are a fixed number of rows on.
+  static __device__ __forceinline__ unsigned offset(int rstride) {
+    return (unsigned)(((int)threadIdx.x / PER_ROW * rstride + (int)threadIdx.x % PER_ROW * V) * (int)sizeof(T));
+  }
+  __device__ __forceinline__ void request(const T* base, int rstride, int rows, unsigned off, int width) {
+    const __amdgpu_buffer_rsrc_t d = tm_rsrc(base, ((long long)(rows - 1) * rstride + width) * (long long)sizeof(T));
+#pragma unroll
+    for (int i = 0; i < COUNT; ++i)
+      v[i] = __builtin_bit_cast(Vec<T, V>, __builtin_amdgcn_raw_buffer_load_b128(d, off, i * (THREADS / PER_ROW) * rstride * (int)sizeof(T), 0));
+  }
   // put(plane, row, column, V halves)
-  template <int R, typename F> __device__ __forceinline__ void lay(F put) {
+  template <int R, typename F> __device__ __forceinline__ void lay(int tid, F put) {
 #pragma unroll
     for (int i = 0; i < COUNT; ++i) {
-      const int at = (int)threadIdx.x + i * THREADS, r = at / PER_ROW, c = at % PER_ROW * V;
+      const int at = tid + i * THREADS, r = at / PER_ROW, c = at % PER_ROW * V;
       if (TOTAL % THREADS != 0 && r >= ROWS) continue;
       if constexpr (R == 1) {
         put(0, r, c, __builtin_bit_cast(Vec<unsigned short, V>, v[i]));
@@ -182,23 +200,38 @@ struct Split {
   int seg;       // rows of a tile, a multiple of L; 0: not split
 };
 
+__device__ __forceinline__ float exp2_of(float v) { return __builtin_amdgcn_exp2f(v); }
+// prefix sum over the 16 lanes of a row: shifts within the row bring in zeros
+template <int N> __device__ __forceinline__ double row_shifted(double v) {
+  const unsigned long long b = __builtin_bit_cast(unsigned long long, v);
+  const unsigned lo = (unsigned)__builtin_amdgcn_update_dpp(0, (int)(unsigned)b, 0x110 + N, 0xf, 0xf, true);
+  const unsigned hi = (unsigned)__builtin_amdgcn_update_dpp(0, (int)(unsigned)(b >> 32), 0x110 + N, 0xf, 0xf, true);
+  return __builtin_bit_cast(double, ((unsigned long long)hi << 32) | lo);
+}
+__device__ __forceinline__ double from_lane(double v, int lane) {
+  const unsigned long long b = __builtin_bit_cast(unsigned long long, v);
+  const unsigned lo = (unsigned)__builtin_amdgcn_readlane((int)(unsigned)b, lane), hi = (unsigned)__builtin_amdgcn_readlane((int)(unsigned)(b >> 32), lane);
+  return __builtin_bit_cast(double, ((unsigned long long)hi << 32) | lo);
+}
+
 // STATES: first pass of a split call, the state every tile adds to a zero state.  Otherwise y (and the final states).
-template <typename T, int NP, bool STATES>
-__global__ __launch_bounds__((ScanShape<T, NP>::THREADS)) void selective_scan_chunk_kernel(const mb_selective_scan_args a, const Split sp) {
+// WHOLE: head_dim is a multiple of 64, d_state is NP and the heads of a group are even: only rows can be missing.
+template <typename T, int NP, bool STATES, bool WHOLE>
+__global__ __launch_bounds__((ScanShape<T, NP>::THREADS), (ScanShape<T, NP>::WAVES)) void selective_scan_chunk_kernel(const mb_selective_scan_args a, const Split sp) {
   typedef ScanShape<T, NP> S;
-  constexpr int V = 16 / sizeof(T), R = S::R, Q = S::Q, L = S::L, HB = S::HB, TT = S::TT, NT = S::NT, PB = S::PB, THREADS = S::THREADS;
+  constexpr int V = 16 / sizeof(T), R = S::R, Q = S::Q, L = S::L, HB = S::HB, TT = S::TT, NT = S::NT, PB = S::PB, PT = S::PT, THREADS = S::THREADS;
   extern __shared__ __attribute__((aligned(16))) char lds_raw[];
   typename S::Lds& m = *(typename S::Lds*)lds_raw;
 
-  const int per_group = a.heads / a.groups, hblocks = (per_group + HB - 1) / HB, pblocks = (a.head_dim + PB - 1) / PB;
+  const int head_dim = a.head_dim, d_state = WHOLE ? NP : a.d_state_dim;
+  const int per_group = a.heads / a.groups, hblocks = (per_group + HB - 1) / HB, pblocks = (head_dim + PB - 1) / PB;
   const int units = a.groups * hblocks * pblocks;
   const unsigned tile = blockIdx.x / units;
-  int u = (int)(blockIdx.x - tile * units);
-  const int pb = u % pblocks;
-  u /= pblocks;
-  const int hb = u % hblocks, group = u / hblocks;
-  const int head0 = group * per_group + hb * HB, live = min(HB, per_group - hb * HB);
-  const int p0 = pb * PB;
+  int unit = (int)(blockIdx.x - tile * units);
+  const int p0 = unit % pblocks * PB;
+  unit /= pblocks;
+  const int hb = unit % hblocks, group = unit / hblocks;
+  const int head0 = group * per_group + hb * HB, live = WHOLE ? HB : min(HB, per_group - hb * HB);
 
   const Rows rows = {a.d_cu_seqlens, a.d_valid, a.batch, a.t};
   const int seg = sp.seg ? sp.seg : max(a.t, 1);
@@ -212,127 +245,198 @@ __global__ __launch_bounds__((ScanShape<T, NP>::THREADS)) void selective_scan_ch
   }
   const int t0 = it.part * seg, t1 = min(it.len, t0 + seg);
   const long long pad = a.d_cu_seqlens ? 0 : it.b;
-  const T* xg = (const T*)a.d_x + pad * a.x_bstride + it.row * a.x_rstride + (long long)head0 * a.head_dim + p0;
-  const T* bg = (const T*)a.d_b + pad * a.b_bstride + it.row * a.b_rstride + (long long)group * a.d_state_dim;
-  const T* cg = (const T*)a.d_c + pad * a.c_bstride + it.row * a.c_rstride + (long long)group * a.d_state_dim;
-  T* yg = (T*)a.d_y + pad * a.y_bstride + it.row * a.y_rstride + (long long)head0 * a.head_dim + p0;
+  const T* xg = (const T*)a.d_x + pad * a.x_bstride + it.row * a.x_rstride + (long long)head0 * head_dim + p0;
+  const T* bg = (const T*)a.d_b + pad * a.b_bstride + it.row * a.b_rstride + (long long)group * d_state;
+  const T* cg = (const T*)a.d_c + pad * a.c_bstride + it.row * a.c_rstride + (long long)group * d_state;
   const long long dtg = pad * a.dt_bstride + it.row * a.dt_rstride;
 
-  const int wave = (int)threadIdx.x >> 6, lane = (int)threadIdx.x & 63, g = lane >> 4, li = lane & 15;
-  const int hh = wave % HB, half = wave / HB, head = head0 + min(hh, live - 1);
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = (int)threadIdx.x & 63, g = lane >> 4, li = lane & 15;
+  const int hh = wave % HB, quarter = wave / HB, head = head0 + min(hh, live - 1);
   const bool mine = hh < live;
-  const int pw = half * 32;  // this wave's columns p0 + pw .. + 31
+  const int pw = quarter * (16 * PT);  // this wave's columns p0 + pw ..
+  T* yg = (T*)a.d_y + pad * a.y_bstride + it.row * a.y_rstride + (long long)head * head_dim + p0 + pw;
 
-  f32x4 h[2][NT];  // [column tile][state tile]: h[n = 16 nt + 4 g + i][p = p0 + pw + 16 pt + li]
-  float* st = nullptr;
-  const long long head_state = (long long)a.head_dim * a.d_state_dim;
-  if (a.d_state && !sp.seg) st = a.d_state + slot * a.state_stride + head * head_state;
-  const float* from = sp.seg ? sp.state + ((long long)tile * a.heads + head) * head_state : st;
-  const bool keep = !STATES && (sp.seg ? true : st && (!a.d_has_state || a.d_has_state[it.b]));
+  // h[pt][2 q + e]: column p0 + pw + 16 pt + li, state columns 32 q + 8 g + 4 e + i
+  f32x4 h[PT][NT];
+  const long long head_state = (long long)head_dim * d_state;
+  float* const pool = a.d_state ? a.d_state + slot * a.state_stride + head * head_state : nullptr;
+  float* const joined = sp.seg ? sp.state + ((long long)tile * a.heads + head) * head_state : nullptr;
+  {
+    const float* from = sp.seg ? joined : pool;
+    const bool keep = !STATES && mine && (sp.seg || (pool && (!a.d_has_state || a.d_has_state[it.b])));
 #pragma unroll
-  for (int pt = 0; pt < 2; ++pt)
+    for (int pt = 0; pt < PT; ++pt)
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      const int p = p0 + pw + 16 * pt + li, n = 16 * nt + 4 * g;
-      const int left = keep && mine && p < a.head_dim ? a.d_state_dim - n : 0;
-      h[pt][nt] = __builtin_bit_cast(f32x4, load_some<float, 4>(from + (long long)p * a.d_state_dim + n, left));
-    }
+      for (int nt = 0; nt < NT; ++nt) {
+        const int p = p0 + pw + 16 * pt + li, n = nt / 2 * 32 + 8 * g + nt % 2 * 4;
+        const int left = keep && (WHOLE || p < head_dim) ? (WHOLE ? 4 : d_state - n) : 0;
+        h[pt][nt] = __builtin_bit_cast(f32x4, load_some<float, 4>(from + (long long)p * d_state + n, left));
+      }
+  }
 
   Stage<T, V, L, NP, THREADS> sb, sc;
   Stage<T, V, L, HB * PB, THREADS> sx;
-  float draw = 0.f;
-  auto request = [&](int t) {
+  // x: two heads' columns p0 .. p0 + 63 are 64 apart where head_dim is 64; further apart the second head's vectors sit head_dim - 64 further on
+  const unsigned off_b = WHOLE ? sb.offset((int)a.b_rstride) : 0, off_c = WHOLE && !STATES ? sc.offset((int)a.c_rstride) : 0;
+  const unsigned off_x = WHOLE ? sx.offset((int)a.x_rstride) + ((int)threadIdx.x % sx.PER_ROW * V / PB) * (head_dim - PB) * (int)sizeof(T) : 0;
+  const unsigned off_y = WHOLE ? (li * (int)a.y_rstride + 4 * g) * (int)sizeof(T) : 0;
+  auto request = [&](int t) {  // behind the last row: zeros without a load, so that no register has to keep an older chunk's values
     const int n = t1 - t;
-    auto col_n = [&](int c, int& left) {
-      left = a.d_state_dim - c;
-      return c;
-    };
-    sb.request(bg + t * a.b_rstride, a.b_rstride, n, col_n);
-    if (!STATES) sc.request(cg + t * a.c_rstride, a.c_rstride, n, col_n);
-    sx.request(xg + t * a.x_rstride, a.x_rstride, n, [&](int c, int& left) {
-      const int i = c / PB, p = c % PB;
-      left = i < live ? a.head_dim - p0 - p : 0;
-      return i * a.head_dim + p;
-    });
-    if (half == 0 && mine && lane < L && lane < n) draw = step_raw(a, dtg + (t + lane) * a.dt_rstride + head);
-  };
-  const float A = a.d_a[head], skip = a.d_d ? a.d_d[head] : 0.f;
-  // everything of a chunk that depends on the step sizes alone, one lane per row
-  double walked = 0.0;  // sum of a over the tile so far: its decay
-  auto scalars = [&](int t) {
-    if (half != 0 || !mine) return;
-    const bool in = lane < L && t + lane < t1;
-    const float d = in ? step_of(a, draw, head) : 0.f;
-    double s = in ? (double)d * (double)A : 0.0;
-#pragma unroll
-    for (int o = 1; o < L; o *= 2) {
-      const double up = __shfl_up(s, o, 64);
-      if (lane >= o) s += up;
+    if constexpr (WHOLE) {
+      sb.request(bg + t * a.b_rstride, (int)a.b_rstride, min(n, L), off_b, NP);
+      if (!STATES) sc.request(cg + t * a.c_rstride, (int)a.c_rstride, min(n, L), off_c, NP);
+      sx.request(xg + t * a.x_rstride, (int)a.x_rstride, min(n, L), off_x, head_dim + PB);
+    } else {
+      auto col_n = [&](int c, int& left) {
+        left = d_state - c;
+        return c;
+      };
+      sb.request(bg + t * a.b_rstride, a.b_rstride, n, col_n);
+      if (!STATES) sc.request(cg + t * a.c_rstride, a.c_rstride, n, col_n);
+      sx.request(xg + t * a.x_rstride, a.x_rstride, n, [&](int c, int& left) {
+        const int i = c / PB, p = c % PB;
+        left = i < live ? head_dim - p0 - p : 0;
+        return i * head_dim + p;
+      });
     }
-    const double before = __shfl(s, (lane & ~15) - 1, 64), tile_end = __shfl(s, lane | 15, 64), end = __shfl(s, L - 1, 64);
-    const double start = lane < 16 ? 0.0 : before;
-    typename S::Head& o = m.head[hh];
+  };
+  auto lay = [&](int tid) {
+    sb.template lay<R>(tid, [&](int q, int r, int c, const Vec<unsigned short, V>& v) { store_lds<V>(&m.b[q][r][c], v); });
+    if (!STATES) sc.template lay<R>(tid, [&](int q, int r, int c, const Vec<unsigned short, V>& v) { store_lds<V>(&m.c[q][r][c], v); });
+    sx.template lay<R>(tid, [&](int q, int r, int c, const Vec<unsigned short, V>& v) { store_lds<V>(&m.x[c / PB][q][r][S::x_col(r, c % PB)], v); });
+  };
+  float A = a.d_a[head];
+  double walked = 0.0;  // sum of d A over the tile so far: its decay
+  // Everything of a chunk that depends on the step sizes alone, one lane per row.  Sums are fp64: a difference of two far prefixes keeps
+  // its bits.  Exponents are base 2 from here on.
+  float draw = 0.f;
+  auto request_step = [&](int t) { draw = lane < min(t1 - t, L) ? step_raw(a, dtg + (t + lane) * a.dt_rstride + head) : 0.f; };
+  auto scalars = [&](int t, int to) {
+    const float d = lane < min(t1 - t, L) ? step_of(a, draw, head) : 0.f;
+    asm("" : "+s"(A));  // (its fp64 copy is not worth registers of the whole loop)
+    double s = (double)d * (double)A * 1.4426950408889634;  // log2(e)
+    if (lane >= min(t1 - t, L)) s = 0.0;  // 0 * A of an infinite A
+    s += row_shifted<1>(s);
+    s += row_shifted<2>(s);
+    s += row_shifted<4>(s);
+    s += row_shifted<8>(s);  // from the start of the tile of 16 rows
+    double start[TT + 1];    // of tile j, from the start of the chunk
+    start[0] = 0.0;
+#pragma unroll
+    for (int j = 0; j < TT; ++j) start[j + 1] = start[j] + from_lane(s, 16 * j + 15);
+    double rest = start[1];
+#pragma unroll
+    for (int j = 1; j < TT; ++j)
+      if (g == j) rest = start[j + 1] - start[j];
+    rest -= s;  // to the end of the tile
+    typename S::Head& o = m.head[to][hh];
     if (lane < L) {
-      const double local = s - start;
-      o.u[lane] = expf((float)local);
-      o.w[lane] = expf((float)(tile_end - s)) * d;
-      o.pre[lane] = expf((float)s);
-      o.cs[lane] = expf((float)(end - s)) * d;
       const float hi = (float)s;
+      o.u[lane] = exp2_of(hi);
+      o.w[lane] = exp2_of((float)rest) * d;
       o.hi[lane] = hi;
       o.lo[lane] = (float)(s - (double)hi);
       o.d[lane] = d;
     }
-    // f[i][j]: from the end of tile i to the start of tile j
-    const int i = lane / TT % TT, j = lane % TT;
-    const double fi = __shfl(s, 16 * i + 15, 64), fj = __shfl(s, j ? 16 * j - 1 : 0, 64);
-    if (lane < TT * TT && i < j) o.f[i][j] = expf((float)(fj - fi));
-    if (lane == 0) o.total = expf((float)end);
-    walked += end;
-  };
-  auto lay = [&]() {
-    sb.template lay<R>([&](int q, int r, int c, const Vec<unsigned short, V>& v) { store_vec<unsigned short, V>(&m.b[q][r][c], v); });
-    if (!STATES) sc.template lay<R>([&](int q, int r, int c, const Vec<unsigned short, V>& v) { store_vec<unsigned short, V>(&m.c[q][r][c], v); });
-    sx.template lay<R>([&](int q, int r, int c, const Vec<unsigned short, V>& v) { store_vec<unsigned short, V>(&m.x[c / PB][q][r][c % PB], v); });
+    if (lane == 0) {
+      // f[i][j]: from the end of tile i to the start of tile j
+#pragma unroll
+      for (int i = 0; i < TT; ++i)
+#pragma unroll
+        for (int j = i + 1; j < TT; ++j) o.f[i][j] = exp2_of((float)(start[j] - start[i + 1]));
+#pragma unroll
+      for (int j = 0; j < TT; ++j) {
+        o.front[j] = exp2_of((float)start[j]);                    // from the start of the chunk to the start of tile j
+        o.back[j] = exp2_of((float)(start[TT] - start[j + 1]));   // from the end of tile j to the end of the chunk
+      }
+      o.total = exp2_of((float)start[TT]);
+    }
+    if (STATES) walked += start[TT];
   };
 
-  if (t0 < t1) request(t0);
-  for (int t = t0; t < t1; t += L) {
-    lay();
-    scalars(t);
+  if (WHOLE) request(t0);
+  const bool stepper = mine && quarter == S::WPH - 1;  // the wave of each head that does this, a chunk ahead of the others' products
+  if (stepper) {
+    request_step(t0);
+    scalars(t0, 0);
+    request_step(t0 + L);
+  }
+  int now = 0;
+  for (int t = t0; t < t1; t += L, now ^= 1) {
+    // The lane number is made new in every chunk: LDS addresses derived from it would otherwise be kept through the whole loop, in registers
+    // that are not there.
+    int fresh = lane;
+    asm volatile("" : "+v"(fresh));
+    const int g = fresh >> 4, li = fresh & 15, lane = fresh, tid = wave * 64 + fresh;
+    if (!WHOLE) request(t);  // masks and addresses of partial columns leave no registers to hold values through the products
+    lay(tid);
     meet();
-    if (t + L < t1) request(t + L);
-
-    f32x4 acc[TT][2];
-    const typename S::Head& hd = m.head[hh];
+    const typename S::Head& hd = m.head[now][hh];
+    if (stepper) {
+      scalars(t + L, now ^ 1);
+      request_step(t + 2 * L);
+    }
+    f32x4 acc[TT][PT];
     if (!STATES) {
-      // G^T, tiles (s tile i <= t tile j), dealt to the waves
+      // G^T tiles (s tile i <= t tile j) dealt to the waves, and from each the M^T tiles of both heads
       for (int k = wave; k < S::GT; k += THREADS / 64) {
-        int j = 0;
-        while ((j + 1) * (j + 2) / 2 <= k) ++j;
-        const int i = k - j * (j + 1) / 2;
-        f32x4 s = {0.f, 0.f, 0.f, 0.f};
+        const int j = k < 1 ? 0 : k < 3 ? 1 : k < 6 ? 2 : 3, i = k - j * (j + 1) / 2;
+        f32x4 gt = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int n = 0; n < NP; n += 32) {
           bf16x8 fa[R], fb[R];
 #pragma unroll
           for (int q = 0; q < R; ++q) {
-            fa[q] = read_row<S::NS>(m.b[q], 16 * i + li, n, g);
-            fb[q] = read_row<S::NS>(m.c[q], 16 * j + li, n, g);
+            fa[q] = *(const bf16x8*)&m.b[q][16 * i + li][n + 8 * g];
+            fb[q] = *(const bf16x8*)&m.c[q][16 * j + li][n + 8 * g];
           }
-          s = mma<R, R, R>(fa, fb, s);
+          gt = mma<R, R, R>(fa, fb, gt);
+          if (n % 64) __builtin_amdgcn_sched_barrier(0);
         }
-        m.g[k][lane] = s;
+#pragma unroll
+        for (int e = 0; e < HB; ++e) {
+          if (!WHOLE && e >= live) break;
+          const typename S::Head& o = m.head[now][e];
+          float v[4];
+          if (i < j) {
+            const f32x4 w = *(const f32x4*)&o.w[16 * i + 4 * g];
+            const float u = o.u[16 * j + li] * o.f[i][j];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) v[r] = gt[r] * (u * w[r]);
+          } else {
+            const f32x4 shi = *(const f32x4*)&o.hi[16 * i + 4 * g], slo = *(const f32x4*)&o.lo[16 * i + 4 * g];
+            const f32x4 d = *(const f32x4*)&o.d[16 * i + 4 * g];
+            const float thi = o.hi[16 * j + li], tlo = o.lo[16 * j + li], skip = a.d_d ? a.d_d[head0 + e] : 0.f;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              // the two differences of hi + lo parts are exact or as good as the exponent's own rounding
+              float c = gt[r] * (exp2_of((thi - shi[r]) + (tlo - slo[r])) * d[r]), diagonal = fmaf(gt[r], d[r], skip);
+              asm("" : "+v"(c), "+v"(diagonal));  // both are computed: selects, not branches per lane
+              v[r] = 4 * g + r < li ? c : 4 * g + r == li ? diagonal : 0.f;
+            }
+          }
+          float x0 = v[0], x1 = v[1], x2 = v[2], x3 = v[3];
+#pragma unroll
+          for (int q = 0; q < Q; ++q) {
+            typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+            const u32x2 w = {pack_bf16(x0, x1), pack_bf16(x2, x3)};
+            m.m[e][k][q][lane] = __builtin_bit_cast(bf16x4, w);
+            x0 -= __uint_as_float(w[0] << 16), x1 -= __uint_as_float(w[0] & 0xffff0000u);
+            x2 -= __uint_as_float(w[1] << 16), x3 -= __uint_as_float(w[1] & 0xffff0000u);
+          }
+        }
       }
       // C h, scaled to each row's distance from the state
       if (mine) {
 #pragma unroll
-        for (int j = 0; j < TT; ++j) acc[j][0] = acc[j][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int j = 0; j < TT; ++j)
+#pragma unroll
+          for (int pt = 0; pt < PT; ++pt) acc[j][pt] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int n = 0; n < NT; n += 2) {
-          bf16x8 fh[2][Q];
+          bf16x8 fh[PT][Q];
 #pragma unroll
-          for (int pt = 0; pt < 2; ++pt) {
+          for (int pt = 0; pt < PT; ++pt) {
             const f32x4 lo = h[pt][n], hi = h[pt][n + 1];
             const float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
             split<Q>(v, fh[pt]);
@@ -341,49 +445,49 @@ __global__ __launch_bounds__((ScanShape<T, NP>::THREADS)) void selective_scan_ch
           for (int j = 0; j < TT; ++j) {
             bf16x8 fc[R];
 #pragma unroll
-            for (int q = 0; q < R; ++q) fc[q] = read_row<S::NS>(m.c[q], 16 * j + li, 16 * n, g);
+            for (int q = 0; q < R; ++q) fc[q] = *(const bf16x8*)&m.c[q][16 * j + li][16 * n + 8 * g];
 #pragma unroll
-            for (int pt = 0; pt < 2; ++pt) acc[j][pt] = mma<Q, R, Q>(fh[pt], fc, acc[j][pt]);
+            for (int pt = 0; pt < PT; ++pt) acc[j][pt] = mma<Q, R, Q>(fh[pt], fc, acc[j][pt]);
           }
+          __builtin_amdgcn_sched_barrier(0);  // keeps the scheduler from requesting every operand at once, which spills
         }
 #pragma unroll
         for (int j = 0; j < TT; ++j) {
-          const float pre = hd.pre[16 * j + li];
+          const float pre = hd.u[16 * j + li] * hd.front[j];
 #pragma unroll
-          for (int pt = 0; pt < 2; ++pt) acc[j][pt] *= pre;
+          for (int pt = 0; pt < PT; ++pt) acc[j][pt] *= pre;
         }
       }
       meet();
     }
     if (mine) {
-      bf16x8 fx[2][L / 32][R];
-      bool any = false;
+      bf16x8 fx[PT][L / 32][R];
 #pragma unroll
-      for (int pt = 0; pt < 2; ++pt)
+      for (int pt = 0; pt < PT; ++pt)
 #pragma unroll
         for (int k = 0; k < L / 32; ++k)
 #pragma unroll
           for (int q = 0; q < R; ++q) {
-            fx[pt][k][q] = read_transposed<S::XS>(m.x[hh][q], 32 * k, pw + 16 * pt, lane);
-            any |= not_finite(fx[pt][k][q]);
+            const int r = 32 * k + 4 * g + (li >> 2), c = pw + 16 * pt + 4 * (li & 3);
+            fx[pt][k][q] = read_transposed(&m.x[hh][q][r][S::x_col(r, c)], &m.x[hh][q][r + 16][S::x_col(r + 16, c)]);
           }
       // h <- total h + B^T (c x)
 #pragma unroll
-      for (int pt = 0; pt < 2; ++pt)
+      for (int pt = 0; pt < PT; ++pt)
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) h[pt][nt] *= hd.total;
 #pragma unroll
       for (int k = 0; k < L / 32; ++k) {
-        const f32x4 c0 = *(const f32x4*)&hd.cs[32 * k + 4 * g], c1 = *(const f32x4*)&hd.cs[32 * k + 16 + 4 * g];
-        bf16x8 fs[2][3];
+        const f32x4 c0 = *(const f32x4*)&hd.w[32 * k + 4 * g] * hd.back[2 * k], c1 = *(const f32x4*)&hd.w[32 * k + 16 + 4 * g] * hd.back[2 * k + 1];
+        bf16x8 fs[PT][3];
 #pragma unroll
-        for (int pt = 0; pt < 2; ++pt) {
+        for (int pt = 0; pt < PT; ++pt) {
           float v[8];
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            float xv = 0.f;
+            float xv = value_of(fx[pt][k][R - 1], i);
 #pragma unroll
-            for (int q = R - 1; q >= 0; --q) xv += value_of(fx[pt][k][q], i);
+            for (int q = R - 2; q >= 0; --q) xv += value_of(fx[pt][k][q], i);
             v[i] = (i < 4 ? c0[i & 3] : c1[i & 3]) * xv;
           }
           split<3>(v, fs[pt]);
@@ -392,90 +496,92 @@ __global__ __launch_bounds__((ScanShape<T, NP>::THREADS)) void selective_scan_ch
         for (int nt = 0; nt < NT; ++nt) {
           bf16x8 fb[R];
 #pragma unroll
-          for (int q = 0; q < R; ++q) fb[q] = read_transposed<S::NS>(m.b[q], 32 * k, 16 * nt, lane);
+          for (int q = 0; q < R; ++q) {
+            const int r = 32 * k + 4 * g + (li >> 2), c = nt / 2 * 32 + nt % 2 * 4 + 8 * (li & 3);
+            fb[q] = read_transposed(&m.b[q][r][c], &m.b[q][r + 16][c]);
+          }
 #pragma unroll
-          for (int pt = 0; pt < 2; ++pt) h[pt][nt] = mma<R, 3, 3>(fb, fs[pt], h[pt][nt]);
+          for (int pt = 0; pt < PT; ++pt) h[pt][nt] = mma<R, 3, 3>(fb, fs[pt], h[pt][nt]);
+          if (nt % 4 == 3) __builtin_amdgcn_sched_barrier(0);
         }
       }
+      // The next chunk is requested here, not before the products above: registers for both do not fit together, and the other workgroup
+      // of the CU has work while it comes.
+      __builtin_amdgcn_sched_barrier(0);
+      if (WHOLE) request(t + L);
+      __builtin_amdgcn_sched_barrier(0);
       if (!STATES) {
         // 0 * NaN in the half of M that is zero would reach rows in front of the NaN: such elements are taken out of the product, and
         // their column's rows from there on are set to NaN below
-        int bad[2] = {L, L};  // first such row of this lane's columns
+        int bad[PT];  // first such row of this lane's columns
+#pragma unroll
+        for (int pt = 0; pt < PT; ++pt) bad[pt] = L;
+        bool any = false;
+#pragma unroll
+        for (int pt = 0; pt < PT; ++pt)
+#pragma unroll
+          for (int k = 0; k < L / 32; ++k) any |= not_finite(fx[pt][k][0]);  // a raw value is finite if its first plane is
         const bool poisoned = __any(any);
         if (poisoned) {
 #pragma unroll
-          for (int pt = 0; pt < 2; ++pt) {
+          for (int pt = 0; pt < PT; ++pt) {
 #pragma unroll
-            for (int k = 0; k < L / 32; ++k)
+            for (int k = 0; k < L / 32; ++k) {
+              u32x4 w[R];
 #pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                bool b = false;
+              for (int q = 0; q < R; ++q) w[q] = __builtin_bit_cast(u32x4, fx[pt][k][q]);
 #pragma unroll
-                for (int q = 0; q < R; ++q) b |= !(fabsf(value_of(fx[pt][k][q], i)) <= 3.4e38f);
-                if (b) {
+              for (int i = 0; i < 8; ++i)
+                if (!(fabsf(value_of(fx[pt][k][0], i)) <= 3.4e38f)) {
                   bad[pt] = min(bad[pt], 32 * k + (i < 4 ? 4 * g + i : 12 + 4 * g + i));
 #pragma unroll
-                  for (int q = 0; q < R; ++q) fx[pt][k][q][i] = (__bf16)0.f;
+                  for (int q = 0; q < R; ++q) w[q][i >> 1] &= i & 1 ? 0x0000ffffu : 0xffff0000u;
                 }
-              }
+#pragma unroll
+              for (int q = 0; q < R; ++q) fx[pt][k][q] = __builtin_bit_cast(bf16x8, w[q]);
+            }
             bad[pt] = min(bad[pt], __shfl_xor(bad[pt], 16, 64));
             bad[pt] = min(bad[pt], __shfl_xor(bad[pt], 32, 64));
           }
         }
+        // rows from the tile's end on are dropped by the descriptor's range check
+        const __amdgpu_buffer_rsrc_t dy = tm_rsrc(yg + t * a.y_rstride, ((long long)(min(t1 - t, L) - 1) * a.y_rstride + 16 * PT) * (long long)sizeof(T));
 #pragma unroll
         for (int j = 0; j < TT; ++j) {
-          const float u = hd.u[16 * j + li], thi = hd.hi[16 * j + li], tlo = hd.lo[16 * j + li];
 #pragma unroll
           for (int k = 0; k <= j / 2; ++k) {
-            float v[8];
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const int i = 2 * k + e;
-              if (i > j) {
-#pragma unroll
-                for (int r = 0; r < 4; ++r) v[4 * e + r] = 0.f;
-                continue;
-              }
-              const f32x4 gt = m.g[j * (j + 1) / 2 + i][lane];
-              if (i < j) {
-                const f32x4 w = *(const f32x4*)&hd.w[16 * i + 4 * g];
-                const float uf = u * hd.f[i][j];
-#pragma unroll
-                for (int r = 0; r < 4; ++r) v[4 * e + r] = gt[r] * (uf * w[r]);
-              } else {
-                const f32x4 shi = *(const f32x4*)&hd.hi[16 * i + 4 * g], slo = *(const f32x4*)&hd.lo[16 * i + 4 * g];
-                const f32x4 d = *(const f32x4*)&hd.d[16 * i + 4 * g];
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                  const int s = 4 * g + r;
-                  // the two differences of hi + lo parts are exact or as good as the exponent's own rounding
-                  float c = gt[r] * (expf((thi - shi[r]) + (tlo - slo[r])) * d[r]);
-                  if (s == li) c = fmaf(gt[r], d[r], skip);
-                  v[4 * e + r] = s <= li ? c : 0.f;
-                }
-              }
-            }
             bf16x8 fm[Q];
-            split<Q>(v, fm);
 #pragma unroll
-            for (int pt = 0; pt < 2; ++pt) acc[j][pt] = mma<R, Q, Q>(fx[pt][k], fm, acc[j][pt]);
+            for (int q = 0; q < Q; ++q) {
+              const int at = j * (j + 1) / 2 + 2 * k;
+              const bf16x4 lo = m.m[hh][at][q][lane];
+              bf16x4 hi = {(__bf16)0.f, (__bf16)0.f, (__bf16)0.f, (__bf16)0.f};
+              if (2 * k + 1 <= j) hi = m.m[hh][at + 1][q][lane];
+              fm[q] = bf16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+            }
+#pragma unroll
+            for (int pt = 0; pt < PT; ++pt) acc[j][pt] = mma<R, Q, Q>(fx[pt][k], fm, acc[j][pt]);
           }
           // y^T tile: row p = 4 g + i, column t = li
           const int row = t + 16 * j + li;
 #pragma unroll
-          for (int pt = 0; pt < 2; ++pt) {
+          for (int pt = 0; pt < PT; ++pt) {
             if (poisoned) {
 #pragma unroll
               for (int r = 0; r < 4; ++r)
                 if (16 * j + li >= __shfl(bad[pt], 4 * g + r, 64)) acc[j][pt][r] = __builtin_nanf("");
             }
-            const int p = p0 + pw + 16 * pt + 4 * g;
-            if (row < t1) {
-              T* dst = yg + row * a.y_rstride + (long long)hh * a.head_dim + pw + 16 * pt + 4 * g;
-              Vec<T, 4> o;
+            const int p = 16 * pt + 4 * g;
+            Vec<T, 4> o;
 #pragma unroll
-              for (int r = 0; r < 4; ++r) o.v[r] = from_f32<T>(acc[j][pt][r]);
-              store_some<T, 4>(dst, o, a.head_dim - p);
+            for (int r = 0; r < 4; ++r) o.v[r] = from_f32<T>(acc[j][pt][r]);
+            if constexpr (WHOLE) {
+              typedef unsigned word __attribute__((ext_vector_type(sizeof(T))));
+              const int more = (16 * j * (int)a.y_rstride + 16 * pt) * (int)sizeof(T);
+              if constexpr (sizeof(T) == 2) __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(word, o), dy, off_y, more, 0);
+              else __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(word, o), dy, off_y, more, 0);
+            } else {
+              if (row < t1) store_some<T, 4>(yg + row * a.y_rstride + p, o, head_dim - p0 - pw - p);
             }
           }
         }
@@ -485,22 +591,23 @@ __global__ __launch_bounds__((ScanShape<T, NP>::THREADS)) void selective_scan_ch
   }
 
   if (STATES) {
-    if (half == 0 && mine && lane == 0) sp.decay[(long long)tile * a.heads + head] = expf((float)walked);
-  } else if (!a.d_state || it.part != parts - 1) {
+    if (stepper && lane == 0) sp.decay[(long long)tile * a.heads + head] = exp2_of((float)walked);
+  } else if (!pool || it.part != parts - 1) {
     return;
   }
   if (!mine) return;
-  float* to = STATES ? sp.state + ((long long)tile * a.heads + head) * head_state : a.d_state + slot * a.state_stride + head * head_state;
+  float* const to = STATES ? joined : pool;
 #pragma unroll
-  for (int pt = 0; pt < 2; ++pt)
+  for (int pt = 0; pt < PT; ++pt)
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const int p = p0 + pw + 16 * pt + li, n = 16 * nt + 4 * g;
-      if (p < a.head_dim) store_some<float, 4>(to + (long long)p * a.d_state_dim + n, __builtin_bit_cast(Vec<float, 4>, h[pt][nt]), a.d_state_dim - n);
+      const int p = p0 + pw + 16 * pt + li, n = nt / 2 * 32 + 8 * g + nt % 2 * 4;
+      if (WHOLE || p < head_dim)
+        store_some<float, 4>(to + (long long)p * d_state + n, __builtin_bit_cast(Vec<float, 4>, h[pt][nt]), WHOLE ? 4 : d_state - n);
     }
 }
 
-template <typename T, int NP, bool STATES> int launch_chunk(const mb_selective_scan_args& a, const Split& sp, hipStream_t s) {
+template <typename T, int NP, bool STATES, bool WHOLE> int launch_chunk(const mb_selective_scan_args& a, const Split& sp, hipStream_t s) {
   typedef ScanShape<T, NP> S;
   static_assert(sizeof(typename S::Lds) <= 160 * 1024, "a chunk has to fit LDS");
   static std::atomic<unsigned long long> attr_done{0};  // per device: the attribute belongs to the function on the current device
@@ -508,7 +615,7 @@ template <typename T, int NP, bool STATES> int launch_chunk(const mb_selective_s
   MB_HIP(hipGetDevice(&dev));
   const unsigned long long bit = dev >= 0 && dev < 64 ? 1ull << dev : 0ull;
   if (!bit || !(attr_done.load(std::memory_order_acquire) & bit)) {
-    MB_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(&selective_scan_chunk_kernel<T, NP, STATES>),
+    MB_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(&selective_scan_chunk_kernel<T, NP, STATES, WHOLE>),
                                hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
     attr_done.fetch_or(bit, std::memory_order_release);
   }
@@ -517,15 +624,29 @@ template <typename T, int NP, bool STATES> int launch_chunk(const mb_selective_s
   const long long units = (long long)a.groups * cdiv(per_group, S::HB) * cdiv(a.head_dim, S::PB);
   const long long grid = tiles_of(rows, sp.seg ? sp.seg : (a.t > 1 ? a.t : 1)) * units;
   MB_REQUIRE(grid < (1ll << 31), "selective_scan: %d items of %d heads are too many for one launch", a.batch, a.heads);
-  hipLaunchKernelGGL((selective_scan_chunk_kernel<T, NP, STATES>), dim3((unsigned)grid), dim3(S::THREADS), sizeof(typename S::Lds), s, a, sp);
+  hipLaunchKernelGGL((selective_scan_chunk_kernel<T, NP, STATES, WHOLE>), dim3((unsigned)grid), dim3(S::THREADS), sizeof(typename S::Lds), s, a, sp);
   MB_HIP(hipGetLastError());
   return MB_OK;
 }
 
+template <typename T, int NP> int chunk_by_shape(const mb_selective_scan_args& a, const Split& sp, bool states, hipStream_t s) {
+  typedef ScanShape<T, NP> S;
+  // WHOLE: no partial columns, rows apart from each other and words aligned (buffer accesses), a chunk within a descriptor's 31 bits
+  auto fits = [&](const void* p, long long rstride, long long bstride, long long width) {
+    return aligned(p, 4) && (rstride * (long long)sizeof(T)) % 4 == 0 && (a.d_cu_seqlens || bstride * (long long)sizeof(T) % 4 == 0) && rstride >= width &&
+           rstride * S::L * (long long)sizeof(T) < (1ll << 31);
+  };
+  const long long wide = (long long)a.heads * a.head_dim, narrow = (long long)a.groups * a.d_state_dim;
+  const bool whole = a.head_dim % S::PB == 0 && a.d_state_dim == NP && a.heads / a.groups % S::HB == 0 && fits(a.d_x, a.x_rstride, a.x_bstride, wide) &&
+                     fits(a.d_y, a.y_rstride, a.y_bstride, wide) && fits(a.d_b, a.b_rstride, a.b_bstride, narrow) &&
+                     fits(a.d_c, a.c_rstride, a.c_bstride, narrow);
+  if (states) return whole ? launch_chunk<T, NP, true, true>(a, sp, s) : launch_chunk<T, NP, true, false>(a, sp, s);
+  return whole ? launch_chunk<T, NP, false, true>(a, sp, s) : launch_chunk<T, NP, false, false>(a, sp, s);
+}
 template <typename T> int chunk_launch(const mb_selective_scan_args& a, const Split& sp, bool states, hipStream_t s) {
-  if (a.d_state_dim <= 64) return states ? launch_chunk<T, 64, true>(a, sp, s) : launch_chunk<T, 64, false>(a, sp, s);
-  if (a.d_state_dim <= 128) return states ? launch_chunk<T, 128, true>(a, sp, s) : launch_chunk<T, 128, false>(a, sp, s);
-  return states ? launch_chunk<T, 256, true>(a, sp, s) : launch_chunk<T, 256, false>(a, sp, s);
+  if (a.d_state_dim <= 64) return chunk_by_shape<T, 64>(a, sp, states, s);
+  if (a.d_state_dim <= 128) return chunk_by_shape<T, 128>(a, sp, states, s);
+  return chunk_by_shape<T, 256>(a, sp, states, s);
 }
 
 // the kernels of one type each, in ssm_scan_{f32,f16,bf16}.hip
