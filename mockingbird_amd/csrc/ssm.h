@@ -49,8 +49,13 @@ template <bool FAST> __device__ __forceinline__ float sigmoid(float v) {
   return 1.f / (1.f + expf(-v));
 }
 
-// softplus without overflow: max(v, 0) + log(1 + exp(-|v|)); NaN stays NaN
-__device__ __forceinline__ float softplus(float v) { return (v > 0.f ? v : 0.f) + log1pf(expf(-fabsf(v))); }
+// softplus without overflow: max(v, 0) + log(1 + e), e = exp(-|v|).  The rounding of 1 + e is taken out again by e / ((1 + e) - 1): a few
+// units in the last place at any v.  NaN stays NaN.
+__device__ __forceinline__ float softplus(float v) {
+  const float e = expf(-fabsf(v)), one = 1.f + e, less = one - 1.f;
+  const float log1p = less == 0.f ? e : logf(one) * (e / less);
+  return (v > 0.f ? v : 0.f) + log1p;
+}
 
 // Rows of one call: packed (cu) or padded (valid).  Everything read from the device is clamped to 0..t, so that no list of row numbers
 // can lead outside the tensors.
@@ -65,38 +70,78 @@ struct Item {
   long long row; // its first row on the packed row axis (0 when padded)
   int part;      // which tile of it
 };
-// Tiles never cross an item.  Packed: item b owns the tile numbers from cu[b] / R + b on.  With s = a R + u and len = c R + v the next
-// item starts at least c + 1 >= ceil(len / R) numbers later, so the ranges are disjoint and every item has a tile 0, also an empty one;
-// t / R + batch numbers cover all.  No prefix sum over the items, and the host needs no lengths.
+// Tiles of R rows never cross an item; an item without rows has one (its state is still to be written).  Without lengths on the device every
+// item has the same number of them.  Otherwise they are numbered without gaps -- a gap would be an idle workgroup, and idle ones that
+// alternate with busy ones in dispatch order land on the same shader engines -- from the lengths themselves: 64 items are summed up at a
+// time by the lanes of each wave.  The host needs no lengths, only the bound tiles_of (the numbers behind the last tile are idle).
 __host__ __device__ inline long long tiles_of(const Rows& r, int R) {
   return r.cu ? (long long)r.t / R + r.batch : (long long)r.batch * (r.t > R ? (r.t + R - 1) / R : 1);
 }
-__device__ __forceinline__ Item item_of(const Rows& r, unsigned tile, int R) {
-  Item it;
+__device__ __forceinline__ int rows_of(const Rows& r, int b, int& first) {
   if (r.cu) {
-    int lo = 0, hi = r.batch - 1;
-    while (lo < hi) {  // the last item whose first tile is <= tile
-      const int mid = (lo + hi + 1) >> 1;
-      const int s = min(max(r.cu[mid], 0), r.t);
-      if (s / R + mid <= (int)tile) lo = mid; else hi = mid - 1;
-    }
-    const int s = min(max(r.cu[lo], 0), r.t), e = min(max(r.cu[lo + 1], s), r.t);
-    it.b = lo; it.len = e - s; it.row = s; it.part = (int)tile - (s / R + lo);
-  } else {
+    first = min(max(r.cu[b], 0), r.t);
+    return min(max(r.cu[b + 1], first), r.t) - first;
+  }
+  first = 0;
+  return r.valid ? min(max(r.valid[b], 0), r.t) : r.t;
+}
+__device__ __forceinline__ int lanes_prefix(int v) {  // inclusive, over the wave
+  const int lane = (int)threadIdx.x & 63;
+#pragma unroll
+  for (int o = 1; o < 64; o *= 2) {
+    const int up = __shfl_up(v, o, 64);
+    v += lane >= o ? up : 0;
+  }
+  return v;
+}
+// part < 0: no such tile.  Every lane of the wave calls it with the same tile.
+__device__ __forceinline__ Item item_of(const Rows& r, unsigned tile, int R) {
+  Item it = {0, 0, 0, -1};
+  if (!r.cu && !r.valid) {
     const unsigned per = r.t > R ? (unsigned)(r.t + R - 1) / R : 1u;
     it.b = (int)(tile / per);
     it.part = (int)(tile - (unsigned)it.b * per);
-    it.len = r.valid ? min(max(r.valid[it.b], 0), r.t) : r.t;
-    it.row = 0;
+    it.len = r.t;
+    return it;
+  }
+  int base = 0;
+  for (int i0 = 0; i0 < r.batch; i0 += 64) {
+    const int i = i0 + ((int)threadIdx.x & 63);
+    int first = 0, len = 0, parts = 0;
+    if (i < r.batch) {
+      len = rows_of(r, i, first);
+      parts = max(1, (len + R - 1) / R);
+    }
+    const int end = base + lanes_prefix(parts);
+    const unsigned long long behind = __ballot(end > (int)tile);
+    if (behind) {
+      const int l = __builtin_amdgcn_readfirstlane(__ffsll((long long)behind) - 1);  // scalars from here on
+      it.b = i0 + l;
+      it.len = __builtin_amdgcn_readlane(len, l);
+      it.row = __builtin_amdgcn_readlane(first, l);
+      it.part = (int)tile - (__builtin_amdgcn_readlane(end, l) - __builtin_amdgcn_readlane(parts, l));
+      return it;
+    }
+    base = __builtin_amdgcn_readlane(end, 63);
   }
   return it;
+}
+// First tile of item b; every lane of the wave calls it with the same b.
+__device__ __forceinline__ int first_tile_of(const Rows& r, int b, int R) {
+  if (!r.cu && !r.valid) return b * (r.t > R ? (r.t + R - 1) / R : 1);
+  int sum = 0;
+  for (int i = (int)threadIdx.x & 63; i < b; i += 64) {
+    int first;
+    sum += max(1, (rows_of(r, i, first) + R - 1) / R);
+  }
+  return __builtin_amdgcn_readlane(lanes_prefix(sum), 63);
 }
 
 // Slot of item b, or -1: outside the pool, or named by an earlier item as well (two updates of one state would race; the first wins).
 // Wave-uniform; every lane of the wave calls it.
 __device__ __forceinline__ int slot_of(const int* slots, int b, int n_slots) {
   if (!slots) return b;
-  const int s = slots[b];
+  const int s = __builtin_amdgcn_readfirstlane(slots[b]);
   if (s < 0 || s >= n_slots) return -1;
   bool twice = false;
   for (int i = (int)(threadIdx.x & 63); i < b; i += 64) twice |= slots[i] == s;

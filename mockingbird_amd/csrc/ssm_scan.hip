@@ -78,18 +78,12 @@ __global__ __launch_bounds__(256) void selective_scan_join_kernel(const mb_selec
     slot = slot_of(a.d_slots, b, a.n_slots);
     if (slot < 0) return;
   }
+  const Rows rows = {a.d_cu_seqlens, a.d_valid, a.batch, a.t};
+  int first;
+  const int parts = (rows_of(rows, b, first) + sp.seg - 1) / sp.seg;
+  if (parts <= 1) return;  // not split: its workgroups read and write the pool themselves
+  const long long tile = first_tile_of(rows, b, sp.seg);
   if (n <= 0) return;
-  long long tile;
-  int len;
-  if (a.d_cu_seqlens) {
-    const int s = min(max(a.d_cu_seqlens[b], 0), a.t);
-    len = min(max(a.d_cu_seqlens[b + 1], s), a.t) - s;
-    tile = s / sp.seg + b;
-  } else {
-    len = a.d_valid ? min(max(a.d_valid[b], 0), a.t) : a.t;
-    tile = (long long)b * (a.t > sp.seg ? (a.t + sp.seg - 1) / sp.seg : 1);
-  }
-  const int parts = max(1, (len + sp.seg - 1) / sp.seg);
   const bool keep = a.d_state && (!a.d_has_state || a.d_has_state[b]);
   Vec<float, 4> h = load_some<float, 4>(a.d_state + slot * a.state_stride + (long long)head * elems + e, keep ? n : 0);
   const long long step = (long long)a.heads * elems;
@@ -134,13 +128,19 @@ template <typename T> int step_by_lanes(const mb_selective_scan_args& a, hipStre
   return launch_step<T, 64>(a, s);
 }
 
-// Rows of a time tile, or 0 for one workgroup walking a whole item.  About 512 workgroups (two per CU) are wanted.  The host does not
-// know the lengths of packed items: it deals out the rows of all together.
+// Rows of a time tile, or 0 for one workgroup walking a whole item.  Splitting costs a second pass over x and B, and states through memory;
+// it pays where the items alone would leave CUs without a workgroup.  The host does not know the lengths of packed items: it deals out the
+// rows of all together, and with enough items splits only those of more than twice the mean length.
 static int rows_per_tile(const mb_selective_scan_args& a) {
   const long long units = (long long)a.groups * cdiv(a.heads / a.groups, 2) * cdiv(a.head_dim, 64);
   const long long all = a.d_cu_seqlens ? a.t : (long long)a.t * a.batch;
-  long long seg = (all * units + 511) / 512;
-  if (seg < 256) seg = 256;
+  const bool full = units * a.batch >= 256;
+  if (full && !a.d_cu_seqlens) return 0;
+  long long seg = (all * units + 511) / 512;  // two workgroups per CU
+  // shorter tiles shorten the walk but move more states: not below 128 rows where a head's state outweighs 64 rows of its x
+  const int least = a.head_dim * a.d_state_dim < 4096 ? 64 : 128;
+  if (seg < least) seg = least;
+  if (full && seg < 2 * all / a.batch) seg = 2 * all / a.batch;
   seg = (seg + 63) / 64 * 64;
   return seg >= a.t ? 0 : (int)seg;
 }

@@ -43,6 +43,18 @@ __device__ __forceinline__ float step_size(const mb_selective_scan_args& a, long
 
 __device__ __forceinline__ float bf16_bits(unsigned short v) { return __uint_as_float((unsigned)v << 16); }
 
+// Schedule of a region: DS_FIRST LDS reads, then MFMAS matrix instructions with up to VALU vector instructions behind each and the rest of
+// the DS LDS reads spread over them.  Without it the conversions of the next operands come in one block, and neither pipe runs beside the other.
+template <int MFMAS, int VALU, int DS, int DS_FIRST> __device__ __forceinline__ void behind_each() {
+  __builtin_amdgcn_sched_group_barrier(0x100, DS_FIRST, 0);
+#pragma unroll
+  for (int i = 0; i < MFMAS; ++i) {
+    if (DS_FIRST + i < DS) __builtin_amdgcn_sched_group_barrier(0x100, (DS - DS_FIRST + MFMAS - 1) / MFMAS, 0);
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    __builtin_amdgcn_sched_group_barrier(0x002, VALU, 0);
+  }
+  __builtin_amdgcn_sched_barrier(0);
+}
 // Planes of 8 values: each the rounded remainder of those before it (Q planes carry 8 Q bits and a sign, the last one rounds).
 // Two values at a time: one packed conversion, and their fp32 value back from its halves.
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
@@ -99,8 +111,8 @@ template <typename T, int NP> struct ScanShape {
   static constexpr int L = R == 1 && NP <= 128 ? 64 : 32;  // rows of a chunk: 64 where two workgroups' LDS and registers hold them
   static constexpr int HB = 2;                             // heads of a workgroup
   static constexpr int PB = 64;                            // columns of a workgroup
-  static constexpr int PT = 1;                             // 16-column tiles of a wave
-  static constexpr int WPH = PB / (16 * PT);               // waves per head
+  static constexpr int WPH = PB / 16;                      // waves per head: 16 columns each
+  static constexpr int CH_PAIRS = R == 1 ? 2 : R == 2 ? 3 : 6, ST_PAIRS = R == 1 ? 3 : R == 2 ? 5 : 6;  // products per operand pair
   static constexpr int THREADS = HB * WPH * 64;
   static constexpr int TT = L / 16;                        // row tiles
   static constexpr int NT = NP / 16;                       // state tiles
@@ -219,7 +231,7 @@ __device__ __forceinline__ double from_lane(double v, int lane) {
 template <typename T, int NP, bool STATES, bool WHOLE>
 __global__ __launch_bounds__((ScanShape<T, NP>::THREADS), (ScanShape<T, NP>::WAVES)) void selective_scan_chunk_kernel(const mb_selective_scan_args a, const Split sp) {
   typedef ScanShape<T, NP> S;
-  constexpr int V = 16 / sizeof(T), R = S::R, Q = S::Q, L = S::L, HB = S::HB, TT = S::TT, NT = S::NT, PB = S::PB, PT = S::PT, THREADS = S::THREADS;
+  constexpr int V = 16 / sizeof(T), R = S::R, Q = S::Q, L = S::L, HB = S::HB, TT = S::TT, NT = S::NT, PB = S::PB, THREADS = S::THREADS;
   extern __shared__ __attribute__((aligned(16))) char lds_raw[];
   typename S::Lds& m = *(typename S::Lds*)lds_raw;
 
@@ -253,24 +265,22 @@ __global__ __launch_bounds__((ScanShape<T, NP>::THREADS), (ScanShape<T, NP>::WAV
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = (int)threadIdx.x & 63, g = lane >> 4, li = lane & 15;
   const int hh = wave % HB, quarter = wave / HB, head = head0 + min(hh, live - 1);
   const bool mine = hh < live;
-  const int pw = quarter * (16 * PT);  // this wave's columns p0 + pw ..
+  const int pw = quarter * 16;  // this wave's columns p0 + pw ..
   T* yg = (T*)a.d_y + pad * a.y_bstride + it.row * a.y_rstride + (long long)head * head_dim + p0 + pw;
 
-  // h[pt][2 q + e]: column p0 + pw + 16 pt + li, state columns 32 q + 8 g + 4 e + i
-  f32x4 h[PT][NT];
+  // h[2 q + e]: column p0 + pw + li, state columns 32 q + 8 g + 4 e + i
+  f32x4 h[NT];
   const long long head_state = (long long)head_dim * d_state;
   float* const pool = a.d_state ? a.d_state + slot * a.state_stride + head * head_state : nullptr;
   float* const joined = sp.seg ? sp.state + ((long long)tile * a.heads + head) * head_state : nullptr;
   {
-    const float* from = sp.seg ? joined : pool;
-    const bool keep = !STATES && mine && (sp.seg || (pool && (!a.d_has_state || a.d_has_state[it.b])));
-#pragma unroll
-    for (int pt = 0; pt < PT; ++pt)
+    const float* from = parts > 1 ? joined : pool;  // an item of one part is not split
+    const bool keep = !STATES && mine && (parts > 1 || (pool && (!a.d_has_state || a.d_has_state[it.b])));
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        const int p = p0 + pw + 16 * pt + li, n = nt / 2 * 32 + 8 * g + nt % 2 * 4;
+        const int p = p0 + pw + li, n = nt / 2 * 32 + 8 * g + nt % 2 * 4;
         const int left = keep && (WHOLE || p < head_dim) ? (WHOLE ? 4 : d_state - n) : 0;
-        h[pt][nt] = __builtin_bit_cast(f32x4, load_some<float, 4>(from + (long long)p * d_state + n, left));
+        h[nt] = __builtin_bit_cast(f32x4, load_some<float, 4>(from + (long long)p * d_state + n, left));
       }
   }
 
@@ -320,15 +330,12 @@ __global__ __launch_bounds__((ScanShape<T, NP>::THREADS), (ScanShape<T, NP>::WAV
     s += row_shifted<2>(s);
     s += row_shifted<4>(s);
     s += row_shifted<8>(s);  // from the start of the tile of 16 rows
-    double start[TT + 1];    // of tile j, from the start of the chunk
-    start[0] = 0.0;
+    double rest = 0.0, sum[TT];  // of tile j
 #pragma unroll
-    for (int j = 0; j < TT; ++j) start[j + 1] = start[j] + from_lane(s, 16 * j + 15);
-    double rest = start[1];
-#pragma unroll
-    for (int j = 1; j < TT; ++j)
-      if (g == j) rest = start[j + 1] - start[j];
-    rest -= s;  // to the end of the tile
+    for (int j = 0; j < TT; ++j) {
+      sum[j] = from_lane(s, 16 * j + 15);
+      if (g == j) rest = sum[j] - s;  // to the end of the tile
+    }
     typename S::Head& o = m.head[to][hh];
     if (lane < L) {
       const float hi = (float)s;
@@ -338,20 +345,28 @@ __global__ __launch_bounds__((ScanShape<T, NP>::THREADS), (ScanShape<T, NP>::WAV
       o.lo[lane] = (float)(s - (double)hi);
       o.d[lane] = d;
     }
+    // decays across whole tiles: products of theirs
+    float by[TT], front = 1.f, back = 1.f;
+#pragma unroll
+    for (int j = 0; j < TT; ++j) by[j] = exp2_of((float)sum[j]);
     if (lane == 0) {
-      // f[i][j]: from the end of tile i to the start of tile j
-#pragma unroll
-      for (int i = 0; i < TT; ++i)
-#pragma unroll
-        for (int j = i + 1; j < TT; ++j) o.f[i][j] = exp2_of((float)(start[j] - start[i + 1]));
 #pragma unroll
       for (int j = 0; j < TT; ++j) {
-        o.front[j] = exp2_of((float)start[j]);                    // from the start of the chunk to the start of tile j
-        o.back[j] = exp2_of((float)(start[TT] - start[j + 1]));   // from the end of tile j to the end of the chunk
+        o.front[j] = front;             // from the start of the chunk to the start of tile j
+        o.back[TT - 1 - j] = back;      // from the end of that tile to the end of the chunk
+        front *= by[j], back *= by[TT - 1 - j];
+        float f = 1.f;                  // from the end of tile j to the start of tile k
+#pragma unroll
+        for (int k = j + 1; k < TT; ++k) {
+          o.f[j][k] = f;
+          f *= by[k];
+        }
       }
-      o.total = exp2_of((float)start[TT]);
+      o.total = front;
     }
-    if (STATES) walked += start[TT];
+    if (STATES)
+#pragma unroll
+      for (int j = 0; j < TT; ++j) walked += sum[j];
   };
 
   if (WHOLE) request(t0);
@@ -376,7 +391,7 @@ __global__ __launch_bounds__((ScanShape<T, NP>::THREADS), (ScanShape<T, NP>::WAV
       scalars(t + L, now ^ 1);
       request_step(t + 2 * L);
     }
-    f32x4 acc[TT][PT];
+    f32x4 acc[TT];
     if (!STATES) {
       // G^T tiles (s tile i <= t tile j) dealt to the waves, and from each the M^T tiles of both heads
       for (int k = wave; k < S::GT; k += THREADS / 64) {
@@ -429,69 +444,65 @@ __global__ __launch_bounds__((ScanShape<T, NP>::THREADS), (ScanShape<T, NP>::WAV
       // C h, scaled to each row's distance from the state
       if (mine) {
 #pragma unroll
-        for (int j = 0; j < TT; ++j)
-#pragma unroll
-          for (int pt = 0; pt < PT; ++pt) acc[j][pt] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int j = 0; j < TT; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+        // the next operand is split between this one's products, a few vector instructions behind each
+        bf16x8 fh[2][Q];
+        auto split_h = [&](int n, bf16x8 (&to)[Q]) {
+          const float v[8] = {h[n][0], h[n][1], h[n][2], h[n][3], h[n + 1][0], h[n + 1][1], h[n + 1][2], h[n + 1][3]};
+          split<Q>(v, to);
+        };
+        split_h(0, fh[0]);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int n = 0; n < NT; n += 2) {
-          bf16x8 fh[PT][Q];
-#pragma unroll
-          for (int pt = 0; pt < PT; ++pt) {
-            const f32x4 lo = h[pt][n], hi = h[pt][n + 1];
-            const float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-            split<Q>(v, fh[pt]);
-          }
+          if (n + 2 < NT) split_h(n + 2, fh[n / 2 + 1 & 1]);
 #pragma unroll
           for (int j = 0; j < TT; ++j) {
             bf16x8 fc[R];
 #pragma unroll
             for (int q = 0; q < R; ++q) fc[q] = *(const bf16x8*)&m.c[q][16 * j + li][16 * n + 8 * g];
-#pragma unroll
-            for (int pt = 0; pt < PT; ++pt) acc[j][pt] = mma<Q, R, Q>(fh[pt], fc, acc[j][pt]);
+            acc[j] = mma<Q, R, Q>(fh[n / 2 & 1], fc, acc[j]);
           }
-          __builtin_amdgcn_sched_barrier(0);  // keeps the scheduler from requesting every operand at once, which spills
+          behind_each<TT * S::CH_PAIRS, 3, TT * R, R>();
         }
 #pragma unroll
         for (int j = 0; j < TT; ++j) {
-          const float pre = hd.u[16 * j + li] * hd.front[j];
-#pragma unroll
-          for (int pt = 0; pt < PT; ++pt) acc[j][pt] *= pre;
+          acc[j] *= hd.u[16 * j + li] * hd.front[j];
         }
       }
       meet();
     }
     if (mine) {
-      bf16x8 fx[PT][L / 32][R];
+      bf16x8 fx[L / 32][R];
+      auto read_x = [&](int k) {
 #pragma unroll
-      for (int pt = 0; pt < PT; ++pt)
+        for (int q = 0; q < R; ++q) {
+          const int r = 32 * k + 4 * g + (li >> 2), c = pw + 4 * (li & 3);
+          fx[k][q] = read_transposed(&m.x[hh][q][r][S::x_col(r, c)], &m.x[hh][q][r + 16][S::x_col(r + 16, c)]);
+        }
+      };
+      auto scale_x = [&](int k, bf16x8 (&to)[3]) {  // c x of rows 32 k .. + 31
+        const f32x4 c0 = *(const f32x4*)&hd.w[32 * k + 4 * g] * hd.back[2 * k], c1 = *(const f32x4*)&hd.w[32 * k + 16 + 4 * g] * hd.back[2 * k + 1];
+        float v[8];
 #pragma unroll
-        for (int k = 0; k < L / 32; ++k)
+        for (int i = 0; i < 8; ++i) {
+          float xv = value_of(fx[k][R - 1], i);
 #pragma unroll
-          for (int q = 0; q < R; ++q) {
-            const int r = 32 * k + 4 * g + (li >> 2), c = pw + 16 * pt + 4 * (li & 3);
-            fx[pt][k][q] = read_transposed(&m.x[hh][q][r][S::x_col(r, c)], &m.x[hh][q][r + 16][S::x_col(r + 16, c)]);
-          }
+          for (int q = R - 2; q >= 0; --q) xv += value_of(fx[k][q], i);
+          v[i] = (i < 4 ? c0[i & 3] : c1[i & 3]) * xv;
+        }
+        split<3>(v, to);
+      };
       // h <- total h + B^T (c x)
+      bf16x8 fs[2][3];
 #pragma unroll
-      for (int pt = 0; pt < PT; ++pt)
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) h[pt][nt] *= hd.total;
+      for (int k = 0; k < L / 32; ++k) read_x(k);
+      scale_x(0, fs[0]);
+      const float total = hd.total;
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int k = 0; k < L / 32; ++k) {
-        const f32x4 c0 = *(const f32x4*)&hd.w[32 * k + 4 * g] * hd.back[2 * k], c1 = *(const f32x4*)&hd.w[32 * k + 16 + 4 * g] * hd.back[2 * k + 1];
-        bf16x8 fs[PT][3];
-#pragma unroll
-        for (int pt = 0; pt < PT; ++pt) {
-          float v[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            float xv = value_of(fx[pt][k][R - 1], i);
-#pragma unroll
-            for (int q = R - 2; q >= 0; --q) xv += value_of(fx[pt][k][q], i);
-            v[i] = (i < 4 ? c0[i & 3] : c1[i & 3]) * xv;
-          }
-          split<3>(v, fs[pt]);
-        }
+        if (k + 1 < L / 32) scale_x(k + 1, fs[k + 1 & 1]);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           bf16x8 fb[R];
@@ -500,10 +511,10 @@ __global__ __launch_bounds__((ScanShape<T, NP>::THREADS), (ScanShape<T, NP>::WAV
             const int r = 32 * k + 4 * g + (li >> 2), c = nt / 2 * 32 + nt % 2 * 4 + 8 * (li & 3);
             fb[q] = read_transposed(&m.b[q][r][c], &m.b[q][r + 16][c]);
           }
-#pragma unroll
-          for (int pt = 0; pt < PT; ++pt) h[pt][nt] = mma<R, 3, 3>(fb, fs[pt], h[pt][nt]);
-          if (nt % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+          if (k == 0) h[nt] *= total;
+          h[nt] = mma<R, 3, 3>(fb, fs[k & 1], h[nt]);
         }
+        behind_each<NT * S::ST_PAIRS, 3, NT * 2 * R, 2 * R>();
       }
       // The next chunk is requested here, not before the products above: registers for both do not fit together, and the other workgroup
       // of the CU has work while it comes.
@@ -513,39 +524,32 @@ __global__ __launch_bounds__((ScanShape<T, NP>::THREADS), (ScanShape<T, NP>::WAV
       if (!STATES) {
         // 0 * NaN in the half of M that is zero would reach rows in front of the NaN: such elements are taken out of the product, and
         // their column's rows from there on are set to NaN below
-        int bad[PT];  // first such row of this lane's columns
-#pragma unroll
-        for (int pt = 0; pt < PT; ++pt) bad[pt] = L;
+        int bad = L;  // first such row of this lane's column
         bool any = false;
 #pragma unroll
-        for (int pt = 0; pt < PT; ++pt)
-#pragma unroll
-          for (int k = 0; k < L / 32; ++k) any |= not_finite(fx[pt][k][0]);  // a raw value is finite if its first plane is
+        for (int k = 0; k < L / 32; ++k) any |= not_finite(fx[k][0]);  // a raw value is finite if its first plane is
         const bool poisoned = __any(any);
         if (poisoned) {
 #pragma unroll
-          for (int pt = 0; pt < PT; ++pt) {
+          for (int k = 0; k < L / 32; ++k) {
+            u32x4 w[R];
 #pragma unroll
-            for (int k = 0; k < L / 32; ++k) {
-              u32x4 w[R];
+            for (int q = 0; q < R; ++q) w[q] = __builtin_bit_cast(u32x4, fx[k][q]);
 #pragma unroll
-              for (int q = 0; q < R; ++q) w[q] = __builtin_bit_cast(u32x4, fx[pt][k][q]);
+            for (int i = 0; i < 8; ++i)
+              if (!(fabsf(value_of(fx[k][0], i)) <= 3.4e38f)) {
+                bad = min(bad, 32 * k + (i < 4 ? 4 * g + i : 12 + 4 * g + i));
 #pragma unroll
-              for (int i = 0; i < 8; ++i)
-                if (!(fabsf(value_of(fx[pt][k][0], i)) <= 3.4e38f)) {
-                  bad[pt] = min(bad[pt], 32 * k + (i < 4 ? 4 * g + i : 12 + 4 * g + i));
+                for (int q = 0; q < R; ++q) w[q][i >> 1] &= i & 1 ? 0x0000ffffu : 0xffff0000u;
+              }
 #pragma unroll
-                  for (int q = 0; q < R; ++q) w[q][i >> 1] &= i & 1 ? 0x0000ffffu : 0xffff0000u;
-                }
-#pragma unroll
-              for (int q = 0; q < R; ++q) fx[pt][k][q] = __builtin_bit_cast(bf16x8, w[q]);
-            }
-            bad[pt] = min(bad[pt], __shfl_xor(bad[pt], 16, 64));
-            bad[pt] = min(bad[pt], __shfl_xor(bad[pt], 32, 64));
+            for (int q = 0; q < R; ++q) fx[k][q] = __builtin_bit_cast(bf16x8, w[q]);
           }
+          bad = min(bad, __shfl_xor(bad, 16, 64));
+          bad = min(bad, __shfl_xor(bad, 32, 64));
         }
         // rows from the tile's end on are dropped by the descriptor's range check
-        const __amdgpu_buffer_rsrc_t dy = tm_rsrc(yg + t * a.y_rstride, ((long long)(min(t1 - t, L) - 1) * a.y_rstride + 16 * PT) * (long long)sizeof(T));
+        const __amdgpu_buffer_rsrc_t dy = tm_rsrc(yg + t * a.y_rstride, ((long long)(min(t1 - t, L) - 1) * a.y_rstride + 16) * (long long)sizeof(T));
 #pragma unroll
         for (int j = 0; j < TT; ++j) {
 #pragma unroll
@@ -559,30 +563,25 @@ __global__ __launch_bounds__((ScanShape<T, NP>::THREADS), (ScanShape<T, NP>::WAV
               if (2 * k + 1 <= j) hi = m.m[hh][at + 1][q][lane];
               fm[q] = bf16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
             }
-#pragma unroll
-            for (int pt = 0; pt < PT; ++pt) acc[j][pt] = mma<R, Q, Q>(fx[pt][k], fm, acc[j][pt]);
+            acc[j] = mma<R, Q, Q>(fx[k], fm, acc[j]);
           }
           // y^T tile: row p = 4 g + i, column t = li
-          const int row = t + 16 * j + li;
+          if (poisoned) {
 #pragma unroll
-          for (int pt = 0; pt < PT; ++pt) {
-            if (poisoned) {
+            for (int r = 0; r < 4; ++r)
+              if (16 * j + li >= __shfl(bad, 4 * g + r, 64)) acc[j][r] = __builtin_nanf("");
+          }
+          Vec<T, 4> o;
 #pragma unroll
-              for (int r = 0; r < 4; ++r)
-                if (16 * j + li >= __shfl(bad[pt], 4 * g + r, 64)) acc[j][pt][r] = __builtin_nanf("");
-            }
-            const int p = 16 * pt + 4 * g;
-            Vec<T, 4> o;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) o.v[r] = from_f32<T>(acc[j][pt][r]);
-            if constexpr (WHOLE) {
-              typedef unsigned word __attribute__((ext_vector_type(sizeof(T))));
-              const int more = (16 * j * (int)a.y_rstride + 16 * pt) * (int)sizeof(T);
-              if constexpr (sizeof(T) == 2) __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(word, o), dy, off_y, more, 0);
-              else __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(word, o), dy, off_y, more, 0);
-            } else {
-              if (row < t1) store_some<T, 4>(yg + row * a.y_rstride + p, o, head_dim - p0 - pw - p);
-            }
+          for (int r = 0; r < 4; ++r) o.v[r] = from_f32<T>(acc[j][r]);
+          if constexpr (WHOLE) {
+            typedef unsigned word __attribute__((ext_vector_type(sizeof(T))));
+            const int more = 16 * j * (int)a.y_rstride * (int)sizeof(T);
+            if constexpr (sizeof(T) == 2) __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(word, o), dy, off_y, more, 0);
+            else __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(word, o), dy, off_y, more, 0);
+          } else {
+            const int row = t + 16 * j + li;
+            if (row < t1) store_some<T, 4>(yg + row * a.y_rstride + 4 * g, o, head_dim - p0 - pw - 4 * g);
           }
         }
       }
@@ -598,12 +597,10 @@ __global__ __launch_bounds__((ScanShape<T, NP>::THREADS), (ScanShape<T, NP>::WAV
   if (!mine) return;
   float* const to = STATES ? joined : pool;
 #pragma unroll
-  for (int pt = 0; pt < PT; ++pt)
-#pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const int p = p0 + pw + 16 * pt + li, n = nt / 2 * 32 + 8 * g + nt % 2 * 4;
+      const int p = p0 + pw + li, n = nt / 2 * 32 + 8 * g + nt % 2 * 4;
       if (WHOLE || p < head_dim)
-        store_some<float, 4>(to + (long long)p * d_state + n, __builtin_bit_cast(Vec<float, 4>, h[pt][nt]), WHOLE ? 4 : d_state - n);
+        store_some<float, 4>(to + (long long)p * d_state + n, __builtin_bit_cast(Vec<float, 4>, h[nt]), WHOLE ? 4 : d_state - n);
     }
 }
 
