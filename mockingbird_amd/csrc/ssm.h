@@ -49,11 +49,17 @@ template <bool FAST> __device__ __forceinline__ float sigmoid(float v) {
   return 1.f / (1.f + expf(-v));
 }
 
+// exp to about an ulp: the product with log2(e) is taken in two parts, the second as a first-order factor.  (Not for |v| beyond 2^7 or so.)
+__device__ __forceinline__ float exp_of(float v) {
+  const float p = v * 1.44269502f, rest = fmaf(v, 1.92596299e-8f, fmaf(v, 1.44269502f, -p));
+  const float e = __builtin_amdgcn_exp2f(p);
+  return fmaf(e, rest * 0.693147182f, e);
+}
 // softplus without overflow: max(v, 0) + log(1 + e), e = exp(-|v|).  The rounding of 1 + e is taken out again by e / ((1 + e) - 1): a few
 // units in the last place at any v.  NaN stays NaN.
 __device__ __forceinline__ float softplus(float v) {
-  const float e = expf(-fabsf(v)), one = 1.f + e, less = one - 1.f;
-  const float log1p = less == 0.f ? e : logf(one) * (e / less);
+  const float e = exp_of(-(fabsf(v) > 120.f ? 120.f : fabsf(v))), one = 1.f + e, less = one - 1.f;
+  const float log1p = less == 0.f ? e : __builtin_amdgcn_logf(one) * 0.693147182f * (e * __builtin_amdgcn_rcpf(less));
   return (v > 0.f ? v : 0.f) + log1p;
 }
 

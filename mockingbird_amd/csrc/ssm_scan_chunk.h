@@ -49,7 +49,9 @@ template <int MFMAS, int VALU, int DS, int DS_FIRST> __device__ __forceinline__ 
   __builtin_amdgcn_sched_group_barrier(0x100, DS_FIRST, 0);
 #pragma unroll
   for (int i = 0; i < MFMAS; ++i) {
-    if (DS_FIRST + i < DS) __builtin_amdgcn_sched_group_barrier(0x100, (DS - DS_FIRST + MFMAS - 1) / MFMAS, 0);
+    constexpr int REST = DS - DS_FIRST;
+    if ((i + 1) * REST / MFMAS - i * REST / MFMAS == 1) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+    if ((i + 1) * REST / MFMAS - i * REST / MFMAS == 2) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
     __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
     __builtin_amdgcn_sched_group_barrier(0x002, VALU, 0);
   }
@@ -167,8 +169,8 @@ template <typename T, int V, int ROWS, int COLS, int THREADS> struct Stage {
   }
   // The same where every column exists: through a buffer descriptor that ends behind row `rows` - 1, whose range check supplies the zeros.
   // One address register for all; the thread's further vectors are a fixed number of rows on.
-  static __device__ __forceinline__ unsigned offset(int rstride) {
-    return (unsigned)(((int)threadIdx.x / PER_ROW * rstride + (int)threadIdx.x % PER_ROW * V) * (int)sizeof(T));
+  static __device__ __forceinline__ unsigned offset(int tid, int rstride) {
+    return (unsigned)((tid / PER_ROW * rstride + tid % PER_ROW * V) * (int)sizeof(T));
   }
   __device__ __forceinline__ void request(const T* base, int rstride, int rows, unsigned off, int width) {
     const __amdgpu_buffer_rsrc_t d = tm_rsrc(base, ((long long)(rows - 1) * rstride + width) * (long long)sizeof(T));
@@ -286,16 +288,14 @@ __global__ __launch_bounds__((ScanShape<T, NP>::THREADS), (ScanShape<T, NP>::WAV
 
   Stage<T, V, L, NP, THREADS> sb, sc;
   Stage<T, V, L, HB * PB, THREADS> sx;
-  // x: two heads' columns p0 .. p0 + 63 are 64 apart where head_dim is 64; further apart the second head's vectors sit head_dim - 64 further on
-  const unsigned off_b = WHOLE ? sb.offset((int)a.b_rstride) : 0, off_c = WHOLE && !STATES ? sc.offset((int)a.c_rstride) : 0;
-  const unsigned off_x = WHOLE ? sx.offset((int)a.x_rstride) + ((int)threadIdx.x % sx.PER_ROW * V / PB) * (head_dim - PB) * (int)sizeof(T) : 0;
-  const unsigned off_y = WHOLE ? (li * (int)a.y_rstride + 4 * g) * (int)sizeof(T) : 0;
-  auto request = [&](int t) {  // behind the last row: zeros without a load, so that no register has to keep an older chunk's values
+  auto request = [&](int t, int tid) {  // behind the last row: zeros without a load, so that no register has to keep an older chunk's values
     const int n = t1 - t;
     if constexpr (WHOLE) {
-      sb.request(bg + t * a.b_rstride, (int)a.b_rstride, min(n, L), off_b, NP);
-      if (!STATES) sc.request(cg + t * a.c_rstride, (int)a.c_rstride, min(n, L), off_c, NP);
-      sx.request(xg + t * a.x_rstride, (int)a.x_rstride, min(n, L), off_x, head_dim + PB);
+      sb.request(bg + t * a.b_rstride, (int)a.b_rstride, min(n, L), sb.offset(tid, (int)a.b_rstride), NP);
+      if (!STATES) sc.request(cg + t * a.c_rstride, (int)a.c_rstride, min(n, L), sc.offset(tid, (int)a.c_rstride), NP);
+      // two heads' columns p0 .. p0 + 63 are next to each other where head_dim is 64; else the second head's are head_dim - 64 further on
+      const unsigned apart = (tid % sx.PER_ROW * V / PB) * (head_dim - PB) * (int)sizeof(T);
+      sx.request(xg + t * a.x_rstride, (int)a.x_rstride, min(n, L), sx.offset(tid, (int)a.x_rstride) + apart, head_dim + PB);
     } else {
       auto col_n = [&](int c, int& left) {
         left = d_state - c;
@@ -324,8 +324,7 @@ __global__ __launch_bounds__((ScanShape<T, NP>::THREADS), (ScanShape<T, NP>::WAV
   auto scalars = [&](int t, int to) {
     const float d = lane < min(t1 - t, L) ? step_of(a, draw, head) : 0.f;
     asm("" : "+s"(A));  // (its fp64 copy is not worth registers of the whole loop)
-    double s = (double)d * (double)A * 1.4426950408889634;  // log2(e)
-    if (lane >= min(t1 - t, L)) s = 0.0;  // 0 * A of an infinite A
+    double s = (double)d * ((double)A * 1.4426950408889634);  // log2(e)
     s += row_shifted<1>(s);
     s += row_shifted<2>(s);
     s += row_shifted<4>(s);
@@ -369,7 +368,7 @@ __global__ __launch_bounds__((ScanShape<T, NP>::THREADS), (ScanShape<T, NP>::WAV
       for (int j = 0; j < TT; ++j) walked += sum[j];
   };
 
-  if (WHOLE) request(t0);
+  if (WHOLE) request(t0, (int)threadIdx.x);
   const bool stepper = mine && quarter == S::WPH - 1;  // the wave of each head that does this, a chunk ahead of the others' products
   if (stepper) {
     request_step(t0);
@@ -383,7 +382,7 @@ __global__ __launch_bounds__((ScanShape<T, NP>::THREADS), (ScanShape<T, NP>::WAV
     int fresh = lane;
     asm volatile("" : "+v"(fresh));
     const int g = fresh >> 4, li = fresh & 15, lane = fresh, tid = wave * 64 + fresh;
-    if (!WHOLE) request(t);  // masks and addresses of partial columns leave no registers to hold values through the products
+    if (!WHOLE) request(t, tid);  // masks and addresses of partial columns leave no registers to hold values through the products
     lay(tid);
     meet();
     const typename S::Head& hd = m.head[now][hh];
@@ -393,9 +392,12 @@ __global__ __launch_bounds__((ScanShape<T, NP>::THREADS), (ScanShape<T, NP>::WAV
     }
     f32x4 acc[TT];
     if (!STATES) {
-      // G^T tiles (s tile i <= t tile j) dealt to the waves, and from each the M^T tiles of both heads
-      for (int k = wave; k < S::GT; k += THREADS / 64) {
-        const int j = k < 1 ? 0 : k < 3 ? 1 : k < 6 ? 2 : 3, i = k - j * (j + 1) / 2;
+      // G^T tiles (s tile i <= t tile j) dealt to the waves, and from each the M^T tiles of both heads: a diagonal tile (about twice the work)
+      // to each of the first TT waves, the others behind them, one each to the last two, which have the step sizes as well
+      constexpr int OFF = TT * (TT - 1) / 2;
+      const int o0 = TT == 4 ? (wave < 6 ? 2 * (wave - 4) : wave - 2) : wave - TT, o1 = TT == 4 && wave < 6 ? o0 + 2 : o0 + 1;
+      for (int k = wave < TT ? -1 : o0; k < (wave < TT ? 0 : min(o1, OFF)); ++k) {
+        const int j = k < 0 ? wave : k < 1 ? 1 : k < 3 ? 2 : 3, i = k < 0 ? wave : k - j * (j - 1) / 2, at = j * (j + 1) / 2 + i;
         f32x4 gt = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int n = 0; n < NP; n += 32) {
@@ -435,7 +437,7 @@ __global__ __launch_bounds__((ScanShape<T, NP>::THREADS), (ScanShape<T, NP>::WAV
           for (int q = 0; q < Q; ++q) {
             typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
             const u32x2 w = {pack_bf16(x0, x1), pack_bf16(x2, x3)};
-            m.m[e][k][q][lane] = __builtin_bit_cast(bf16x4, w);
+            m.m[e][at][q][lane] = __builtin_bit_cast(bf16x4, w);
             x0 -= __uint_as_float(w[0] << 16), x1 -= __uint_as_float(w[0] & 0xffff0000u);
             x2 -= __uint_as_float(w[1] << 16), x3 -= __uint_as_float(w[1] & 0xffff0000u);
           }
@@ -473,30 +475,29 @@ __global__ __launch_bounds__((ScanShape<T, NP>::THREADS), (ScanShape<T, NP>::WAV
       meet();
     }
     if (mine) {
-      bf16x8 fx[L / 32][R];
-      auto read_x = [&](int k) {
+      auto read_x = [&](int k, bf16x8 (&to)[R]) {  // rows 32 k .. + 31 of this lane's column
 #pragma unroll
         for (int q = 0; q < R; ++q) {
           const int r = 32 * k + 4 * g + (li >> 2), c = pw + 4 * (li & 3);
-          fx[k][q] = read_transposed(&m.x[hh][q][r][S::x_col(r, c)], &m.x[hh][q][r + 16][S::x_col(r + 16, c)]);
+          to[q] = read_transposed(&m.x[hh][q][r][S::x_col(r, c)], &m.x[hh][q][r + 16][S::x_col(r + 16, c)]);
         }
       };
-      auto scale_x = [&](int k, bf16x8 (&to)[3]) {  // c x of rows 32 k .. + 31
+      auto scale_x = [&](int k, bf16x8 (&to)[3]) {  // c x
         const f32x4 c0 = *(const f32x4*)&hd.w[32 * k + 4 * g] * hd.back[2 * k], c1 = *(const f32x4*)&hd.w[32 * k + 16 + 4 * g] * hd.back[2 * k + 1];
+        bf16x8 x[R];
+        read_x(k, x);
         float v[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          float xv = value_of(fx[k][R - 1], i);
+          float xv = value_of(x[R - 1], i);
 #pragma unroll
-          for (int q = R - 2; q >= 0; --q) xv += value_of(fx[k][q], i);
+          for (int q = R - 2; q >= 0; --q) xv += value_of(x[q], i);
           v[i] = (i < 4 ? c0[i & 3] : c1[i & 3]) * xv;
         }
         split<3>(v, to);
       };
       // h <- total h + B^T (c x)
       bf16x8 fs[2][3];
-#pragma unroll
-      for (int k = 0; k < L / 32; ++k) read_x(k);
       scale_x(0, fs[0]);
       const float total = hd.total;
       __builtin_amdgcn_sched_barrier(0);
@@ -514,20 +515,25 @@ __global__ __launch_bounds__((ScanShape<T, NP>::THREADS), (ScanShape<T, NP>::WAV
           if (k == 0) h[nt] *= total;
           h[nt] = mma<R, 3, 3>(fb, fs[k & 1], h[nt]);
         }
-        behind_each<NT * S::ST_PAIRS, 3, NT * 2 * R, 2 * R>();
+        if (k + 1 < L / 32) behind_each<NT * S::ST_PAIRS, 3, NT * 2 * R + 2 * R + 3, 4 * R>();
+        else behind_each<NT * S::ST_PAIRS, 3, NT * 2 * R, 4 * R>();
       }
       // The next chunk is requested here, not before the products above: registers for both do not fit together, and the other workgroup
       // of the CU has work while it comes.
       __builtin_amdgcn_sched_barrier(0);
-      if (WHOLE) request(t + L);
+      if (WHOLE) request(t + L, tid);
       __builtin_amdgcn_sched_barrier(0);
       if (!STATES) {
         // 0 * NaN in the half of M that is zero would reach rows in front of the NaN: such elements are taken out of the product, and
         // their column's rows from there on are set to NaN below
         int bad = L;  // first such row of this lane's column
         bool any = false;
+        bf16x8 fx[L / 32][R];
 #pragma unroll
-        for (int k = 0; k < L / 32; ++k) any |= not_finite(fx[k][0]);  // a raw value is finite if its first plane is
+        for (int k = 0; k < L / 32; ++k) {
+          read_x(k, fx[k]);
+          any |= not_finite(fx[k][0]);  // a raw value is finite if its first plane is
+        }
         const bool poisoned = __any(any);
         if (poisoned) {
 #pragma unroll
@@ -548,6 +554,7 @@ __global__ __launch_bounds__((ScanShape<T, NP>::THREADS), (ScanShape<T, NP>::WAV
           bad = min(bad, __shfl_xor(bad, 16, 64));
           bad = min(bad, __shfl_xor(bad, 32, 64));
         }
+        const unsigned off_y = (li * (int)a.y_rstride + 4 * g) * (int)sizeof(T);
         // rows from the tile's end on are dropped by the descriptor's range check
         const __amdgpu_buffer_rsrc_t dy = tm_rsrc(yg + t * a.y_rstride, ((long long)(min(t1 - t, L) - 1) * a.y_rstride + 16) * (long long)sizeof(T));
 #pragma unroll
@@ -565,12 +572,18 @@ __global__ __launch_bounds__((ScanShape<T, NP>::THREADS), (ScanShape<T, NP>::WAV
             }
             acc[j] = mma<R, Q, Q>(fx[k], fm, acc[j]);
           }
-          // y^T tile: row p = 4 g + i, column t = li
-          if (poisoned) {
+          if (j % 2) __builtin_amdgcn_sched_barrier(0);
+        }
+        // y^T tiles: row p = 4 g + i, column t = li
+        if (poisoned) {
+#pragma unroll
+          for (int j = 0; j < TT; ++j)
 #pragma unroll
             for (int r = 0; r < 4; ++r)
               if (16 * j + li >= __shfl(bad, 4 * g + r, 64)) acc[j][r] = __builtin_nanf("");
-          }
+        }
+#pragma unroll
+        for (int j = 0; j < TT; ++j) {
           Vec<T, 4> o;
 #pragma unroll
           for (int r = 0; r < 4; ++r) o.v[r] = from_f32<T>(acc[j][r]);
