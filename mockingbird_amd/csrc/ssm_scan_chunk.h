@@ -34,12 +34,14 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ float step_raw(const mb_selective_scan_args& a, long long at) {
   return a.dt_dtype == MB_F32 ? ((const float*)a.d_dt)[at] : a.dt_dtype == MB_F16 ? to_f32(((const f16*)a.d_dt)[at]) : to_f32(((const bf16*)a.d_dt)[at]);
 }
-__device__ __forceinline__ float step_of(const mb_selective_scan_args& a, float d, int head) {
-  if (a.d_dt_bias) d += a.d_dt_bias[head];
+__device__ __forceinline__ float step_of(const mb_selective_scan_args& a, float d, float bias) {
+  d += bias;
   if (a.dt_softplus) d = softplus(d);
   return d < a.dt_min ? a.dt_min : d > a.dt_max ? a.dt_max : d;  // NaN stays NaN
 }
-__device__ __forceinline__ float step_size(const mb_selective_scan_args& a, long long at, int head) { return step_of(a, step_raw(a, at), head); }
+__device__ __forceinline__ float step_size(const mb_selective_scan_args& a, long long at, int head) {
+  return step_of(a, step_raw(a, at), a.d_dt_bias ? a.d_dt_bias[head] : 0.f);
+}
 
 __device__ __forceinline__ float bf16_bits(unsigned short v) { return __uint_as_float((unsigned)v << 16); }
 
@@ -107,7 +109,7 @@ __device__ __forceinline__ f32x4 mma(const bf16x8 (&a)[QA], const bf16x8 (&b)[QB
   return acc;
 }
 
-template <typename T, int NP> struct ScanShape {
+template <typename T, int NP, bool STATES> struct ScanShape {
   static constexpr int R = sizeof(T) == 4 ? 3 : std::is_same<T, f16>::value ? 2 : 1;  // raw planes
   static constexpr int Q = R == 3 ? 3 : 2;                                             // planes of M and h
   static constexpr int L = R == 1 && NP <= 128 ? 64 : 32;  // rows of a chunk: 64 where two workgroups' LDS and registers hold them
@@ -124,10 +126,14 @@ template <typename T, int NP> struct ScanShape {
   static __device__ __forceinline__ int x_col(int r, int c) { return c ^ 16 * (r >> 1 & 1); }
   static constexpr int GT = TT * (TT + 1) / 2;             // causal tiles of G
   struct alignas(16) Head { float u[L], w[L], hi[L], lo[L], d[L], f[TT][TT], front[TT], back[TT], total; };
-  struct Lds {
-    unsigned short b[R][L][NS], c[R][L][NS], x[HB][R][L][PB];
-    bf16x4 m[HB][GT][Q][64];
-    Head head[2][HB];  // of this chunk and the next
+  // Step-size terms of HEADS chunks.  The states' pass, which needs no C and no M, has room for 8: every wave of a head does one of the next
+  // four chunks at a time.  The other pass keeps this chunk's and the next one's, which one wave of each head does.
+  static constexpr int HEADS = STATES ? 2 * WPH : 2;
+  struct LdsY { unsigned short c[R][L][NS]; bf16x4 m[HB][GT][Q][64]; };
+  struct LdsStates { double walked[HB][WPH]; };
+  struct Lds : std::conditional<STATES, LdsStates, LdsY>::type {
+    unsigned short b[R][L][NS], x[HB][R][L][PB];
+    Head head[HEADS][HB];
   };
   static constexpr int WAVES = (sizeof(Lds) <= 80 * 1024 ? 2 : 1) * THREADS / 256;  // per SIMD, of the workgroups that share a CU
 };
@@ -173,7 +179,8 @@ template <typename T, int V, int ROWS, int COLS, int THREADS> struct Stage {
     return (unsigned)((tid / PER_ROW * rstride + tid % PER_ROW * V) * (int)sizeof(T));
   }
   __device__ __forceinline__ void request(const T* base, int rstride, int rows, unsigned off, int width) {
-    const __amdgpu_buffer_rsrc_t d = tm_rsrc(base, ((long long)(rows - 1) * rstride + width) * (long long)sizeof(T));
+    // (31 bits hold it: the host looked)
+    const __amdgpu_buffer_rsrc_t d = tm_rsrc(base, rows > 0 ? ((rows - 1) * rstride + width) * (int)sizeof(T) : 0);
 #pragma unroll
     for (int i = 0; i < COUNT; ++i)
       v[i] = __builtin_bit_cast(Vec<T, V>, __builtin_amdgcn_raw_buffer_load_b128(d, off, i * (THREADS / PER_ROW) * rstride * (int)sizeof(T), 0));
@@ -231,8 +238,8 @@ __device__ __forceinline__ double from_lane(double v, int lane) {
 // STATES: first pass of a split call, the state every tile adds to a zero state.  Otherwise y (and the final states).
 // WHOLE: head_dim is a multiple of 64, d_state is NP and the heads of a group are even: only rows can be missing.
 template <typename T, int NP, bool STATES, bool WHOLE>
-__global__ __launch_bounds__((ScanShape<T, NP>::THREADS), (ScanShape<T, NP>::WAVES)) void selective_scan_chunk_kernel(const mb_selective_scan_args a, const Split sp) {
-  typedef ScanShape<T, NP> S;
+__global__ __launch_bounds__((ScanShape<T, NP, STATES>::THREADS), (ScanShape<T, NP, STATES>::WAVES)) void selective_scan_chunk_kernel(const mb_selective_scan_args a, const Split sp) {
+  typedef ScanShape<T, NP, STATES> S;
   constexpr int V = 16 / sizeof(T), R = S::R, Q = S::Q, L = S::L, HB = S::HB, TT = S::TT, NT = S::NT, PB = S::PB, THREADS = S::THREADS;
   extern __shared__ __attribute__((aligned(16))) char lds_raw[];
   typename S::Lds& m = *(typename S::Lds*)lds_raw;
@@ -312,17 +319,23 @@ __global__ __launch_bounds__((ScanShape<T, NP>::THREADS), (ScanShape<T, NP>::WAV
   };
   auto lay = [&](int tid) {
     sb.template lay<R>(tid, [&](int q, int r, int c, const Vec<unsigned short, V>& v) { store_lds<V>(&m.b[q][r][c], v); });
-    if (!STATES) sc.template lay<R>(tid, [&](int q, int r, int c, const Vec<unsigned short, V>& v) { store_lds<V>(&m.c[q][r][c], v); });
+    if constexpr (!STATES) sc.template lay<R>(tid, [&](int q, int r, int c, const Vec<unsigned short, V>& v) { store_lds<V>(&m.c[q][r][c], v); });
     sx.template lay<R>(tid, [&](int q, int r, int c, const Vec<unsigned short, V>& v) { store_lds<V>(&m.x[c / PB][q][r][S::x_col(r, c % PB)], v); });
   };
-  float A = a.d_a[head];
+  // scalars of the heads, read once: inside the loop they would be loads behind its stores
+  auto scalar = [&](const float* p, int at) { return __uint_as_float(__builtin_amdgcn_readfirstlane(p ? __float_as_uint(p[at]) : 0u)); };
+  float A = scalar(a.d_a, head);
+  const float bias = scalar(a.d_dt_bias, head);
+  float skips[HB];
+#pragma unroll
+  for (int e = 0; e < HB; ++e) skips[e] = STATES ? 0.f : scalar(a.d_d, head0 + min(e, live - 1));
   double walked = 0.0;  // sum of d A over the tile so far: its decay
   // Everything of a chunk that depends on the step sizes alone, one lane per row.  Sums are fp64: a difference of two far prefixes keeps
   // its bits.  Exponents are base 2 from here on.
   float draw = 0.f;
   auto request_step = [&](int t) { draw = lane < min(t1 - t, L) ? step_raw(a, dtg + (t + lane) * a.dt_rstride + head) : 0.f; };
   auto scalars = [&](int t, int to) {
-    const float d = lane < min(t1 - t, L) ? step_of(a, draw, head) : 0.f;
+    const float d = lane < min(t1 - t, L) ? step_of(a, draw, bias) : 0.f;
     asm("" : "+s"(A));  // (its fp64 copy is not worth registers of the whole loop)
     double s = (double)d * ((double)A * 1.4426950408889634);  // log2(e)
     s += row_shifted<1>(s);
@@ -369,14 +382,17 @@ __global__ __launch_bounds__((ScanShape<T, NP>::THREADS), (ScanShape<T, NP>::WAV
   };
 
   if (WHOLE) request(t0, (int)threadIdx.x);
-  const bool stepper = mine && quarter == S::WPH - 1;  // the wave of each head that does this, a chunk ahead of the others' products
-  if (stepper) {
-    request_step(t0);
-    scalars(t0, 0);
-    request_step(t0 + L);
+  constexpr int HEADS = S::HEADS, FOUR = S::WPH;
+  const bool stepper = mine && quarter == FOUR - 1;  // the wave of each head that does this, a chunk ahead of the others' products
+  if (STATES ? mine : stepper) {
+    const int first = STATES ? quarter : 0, next = STATES ? FOUR : 1;
+    request_step(t0 + first * L);
+    scalars(t0 + first * L, first);
+    request_step(t0 + (first + next) * L);
   }
-  int now = 0;
-  for (int t = t0; t < t1; t += L, now ^= 1) {
+  int chunk = 0;
+  for (int t = t0; t < t1; t += L, ++chunk) {
+    const int now = chunk % HEADS;
     // The lane number is made new in every chunk: LDS addresses derived from it would otherwise be kept through the whole loop, in registers
     // that are not there.
     int fresh = lane;
@@ -386,17 +402,22 @@ __global__ __launch_bounds__((ScanShape<T, NP>::THREADS), (ScanShape<T, NP>::WAV
     lay(tid);
     meet();
     const typename S::Head& hd = m.head[now][hh];
-    if (stepper) {
+    if constexpr (STATES) {
+      if (mine && chunk % FOUR == 0) {
+        scalars(t + (FOUR + quarter) * L, (chunk + FOUR + quarter) % HEADS);
+        request_step(t + (2 * FOUR + quarter) * L);
+      }
+    } else if (stepper) {
       scalars(t + L, now ^ 1);
       request_step(t + 2 * L);
     }
+
     f32x4 acc[TT];
-    if (!STATES) {
-      // G^T tiles (s tile i <= t tile j) dealt to the waves, and from each the M^T tiles of both heads: a diagonal tile (about twice the work)
-      // to each of the first TT waves, the others behind them, one each to the last two, which have the step sizes as well
+    if constexpr (!STATES) {
+      // G^T tiles (s tile i <= t tile j) dealt to the waves, and from each the M^T tiles of both heads: a diagonal tile to each of the first
+      // TT waves, the others to the first 6 (the last two have the step sizes)
       constexpr int OFF = TT * (TT - 1) / 2;
-      const int o0 = TT == 4 ? (wave < 6 ? 2 * (wave - 4) : wave - 2) : wave - TT, o1 = TT == 4 && wave < 6 ? o0 + 2 : o0 + 1;
-      for (int k = wave < TT ? -1 : o0; k < (wave < TT ? 0 : min(o1, OFF)); ++k) {
+      for (int k = wave < TT ? -1 : wave; k < OFF; k = k < 0 && wave < OFF ? wave : OFF) {
         const int j = k < 0 ? wave : k < 1 ? 1 : k < 3 ? 2 : 3, i = k < 0 ? wave : k - j * (j - 1) / 2, at = j * (j + 1) / 2 + i;
         f32x4 gt = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -423,7 +444,7 @@ __global__ __launch_bounds__((ScanShape<T, NP>::THREADS), (ScanShape<T, NP>::WAV
           } else {
             const f32x4 shi = *(const f32x4*)&o.hi[16 * i + 4 * g], slo = *(const f32x4*)&o.lo[16 * i + 4 * g];
             const f32x4 d = *(const f32x4*)&o.d[16 * i + 4 * g];
-            const float thi = o.hi[16 * j + li], tlo = o.lo[16 * j + li], skip = a.d_d ? a.d_d[head0 + e] : 0.f;
+            const float thi = o.hi[16 * j + li], tlo = o.lo[16 * j + li], skip = skips[e];
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
               // the two differences of hi + lo parts are exact or as good as the exponent's own rounding
@@ -523,7 +544,7 @@ __global__ __launch_bounds__((ScanShape<T, NP>::THREADS), (ScanShape<T, NP>::WAV
       __builtin_amdgcn_sched_barrier(0);
       if (WHOLE) request(t + L, tid);
       __builtin_amdgcn_sched_barrier(0);
-      if (!STATES) {
+      if constexpr (!STATES) {
         // 0 * NaN in the half of M that is zero would reach rows in front of the NaN: such elements are taken out of the product, and
         // their column's rows from there on are set to NaN below
         int bad = L;  // first such row of this lane's column
@@ -556,7 +577,7 @@ __global__ __launch_bounds__((ScanShape<T, NP>::THREADS), (ScanShape<T, NP>::WAV
         }
         const unsigned off_y = (li * (int)a.y_rstride + 4 * g) * (int)sizeof(T);
         // rows from the tile's end on are dropped by the descriptor's range check
-        const __amdgpu_buffer_rsrc_t dy = tm_rsrc(yg + t * a.y_rstride, ((long long)(min(t1 - t, L) - 1) * a.y_rstride + 16) * (long long)sizeof(T));
+        const __amdgpu_buffer_rsrc_t dy = tm_rsrc(yg + t * a.y_rstride, ((min(t1 - t, L) - 1) * (int)a.y_rstride + 16) * (int)sizeof(T));
 #pragma unroll
         for (int j = 0; j < TT; ++j) {
 #pragma unroll
@@ -603,7 +624,16 @@ __global__ __launch_bounds__((ScanShape<T, NP>::THREADS), (ScanShape<T, NP>::WAV
   }
 
   if (STATES) {
-    if (stepper && lane == 0) sp.decay[(long long)tile * a.heads + head] = exp2_of((float)walked);
+    if constexpr (STATES) {  // each wave has summed up its own chunks
+      if (mine && lane == 0) m.walked[hh][quarter] = walked;
+      meet();
+      if (stepper && lane == 0) {
+        double sum = 0.0;
+#pragma unroll
+        for (int i = 0; i < FOUR; ++i) sum += m.walked[hh][i];
+        sp.decay[(long long)tile * a.heads + head] = exp2_of((float)sum);
+      }
+    }
   } else if (!pool || it.part != parts - 1) {
     return;
   }
@@ -618,7 +648,7 @@ __global__ __launch_bounds__((ScanShape<T, NP>::THREADS), (ScanShape<T, NP>::WAV
 }
 
 template <typename T, int NP, bool STATES, bool WHOLE> int launch_chunk(const mb_selective_scan_args& a, const Split& sp, hipStream_t s) {
-  typedef ScanShape<T, NP> S;
+  typedef ScanShape<T, NP, STATES> S;
   static_assert(sizeof(typename S::Lds) <= 160 * 1024, "a chunk has to fit LDS");
   static std::atomic<unsigned long long> attr_done{0};  // per device: the attribute belongs to the function on the current device
   int dev = 0;
@@ -640,7 +670,7 @@ template <typename T, int NP, bool STATES, bool WHOLE> int launch_chunk(const mb
 }
 
 template <typename T, int NP> int chunk_by_shape(const mb_selective_scan_args& a, const Split& sp, bool states, hipStream_t s) {
-  typedef ScanShape<T, NP> S;
+  typedef ScanShape<T, NP, false> S;
   // WHOLE: no partial columns, rows apart from each other and words aligned (buffer accesses), a chunk within a descriptor's 31 bits
   auto fits = [&](const void* p, long long rstride, long long bstride, long long width) {
     return aligned(p, 4) && (rstride * (long long)sizeof(T)) % 4 == 0 && (a.d_cu_seqlens || bstride * (long long)sizeof(T) % 4 == 0) && rstride >= width &&
