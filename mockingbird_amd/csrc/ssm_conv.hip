@@ -8,7 +8,7 @@ namespace ssm {
 // The taps of V channels: one run of V * K floats.
 template <int K, int V> __device__ __forceinline__ void load_taps(const float* w, int n, float (&out)[V][K]) {
   if (n >= V) {
-    constexpr int Q = V * K / 4;  // V is 4 or 8
+    constexpr int Q = V * K / 4;
     Vec<float, 4> q[Q];
 #pragma unroll
     for (int i = 0; i < Q; ++i) q[i] = load_vec<float, 4>(w + 4 * i);
@@ -24,12 +24,15 @@ template <int K, int V> __device__ __forceinline__ void load_taps(const float* w
   }
 }
 
-// A thread takes V channels (16 bytes of them) of R rows, cx threads side by side and 256 / cx runs of R rows behind each other.  Memory-
-// bound: each row is read once (a run reads K - 1 more) and the window slides through registers; U rows are requested at a time.
+// A thread takes 4 channels of R rows, cx threads side by side and 256 / cx runs of R rows behind each other.  Memory-bound: each row is
+// read once (a run reads K - 1 more) and the window slides through registers; U rows are requested at a time.  8 channels of a 16-bit type
+// (16 bytes) need 146 registers for window and taps and run at 2.7 TB/s for want of waves, 4 channels at 5.0 TB/s (16 k rows of 4352
+// channels, 4 taps: 108 and 58 us); rows of fp32 are 16 bytes either way.  Runs of 16 to 64 rows differ by 5 %.
+constexpr int CONV_V = 4;
 template <typename T, int K>
 __global__ __launch_bounds__(256) void causal_conv1d_kernel(const mb_causal_conv1d_args a, int cx, int R) {
   constexpr bool FAST = sizeof(T) == 2;
-  constexpr int V = 16 / sizeof(T), U = 4;
+  constexpr int V = CONV_V, U = 4;
   const int ci = threadIdx.x & (cx - 1), rg = threadIdx.x / cx, groups = 256 / cx;
   const int blocks_c = (a.channels + cx * V - 1) / (cx * V);
   const unsigned tile = blockIdx.x / blocks_c;
@@ -148,7 +151,7 @@ template <typename T, int K> int launch_conv(const mb_causal_conv1d_args& a, boo
     MB_REQUIRE(grid < (1ll << 31), "causal_conv1d_step: %d items of %d channels are too many for one launch", a.batch, a.channels);
     hipLaunchKernelGGL((causal_conv1d_step_kernel<T, K>), dim3((unsigned)grid), dim3(64), 0, s, a);
   } else {
-    const int nv = cdiv(a.channels, 16 / (int)sizeof(T));
+    const int nv = cdiv(a.channels, CONV_V);
     int cx = 16;
     while (cx < 256 && cx < nv) cx *= 2;
     // longer runs read fewer rows twice; shorter ones give every CU several workgroups

@@ -167,6 +167,8 @@ static int check_scan(const char* name, const mb_selective_scan_args* a, bool st
   MB_REQUIRE(a->groups >= 1 && a->heads % a->groups == 0, "%s: %d heads in %d groups", name, a->heads, a->groups);
   MB_REQUIRE(a->dt_min <= a->dt_max, "%s: dt_min %g, dt_max %g", name, a->dt_min, a->dt_max);  // refuses NaN as well
   if (a->batch == 0 || a->heads == 0) return MB_OK;
+  MB_REQUIRE((long long)a->batch * a->heads < (1ll << 31) && (a->d_cu_seqlens || (long long)a->batch * (step ? 1 : a->t) < (1ll << 40)),
+             "%s: %d items of %d rows and %d heads are too many for one launch", name, a->batch, a->t, a->heads);
   MB_REQUIRE(a->d_a, "%s: no A", name);
   MB_REQUIRE((a->d_x && a->d_y && a->d_dt && a->d_b && a->d_c) || (!step && a->t == 0), "%s: null x, y, dt, B or C", name);
   MB_REQUIRE(!step || a->d_state, "%s: a step needs a state pool", name);
@@ -214,7 +216,7 @@ static int run_step(const mb_selective_scan_args* a, hipStream_t s) {
 
 extern "C" size_t mb_selective_scan_workspace_bytes(const mb_selective_scan_args* a) {
   using namespace mb::ssm;
-  if (!a || a->batch <= 0 || a->heads <= 0 || a->t <= 0 || a->groups <= 0 || a->head_dim <= 0 || a->d_state_dim <= 0) return 0;
+  if (check_scan("selective_scan_workspace_bytes", a, false) <= 0 || a->t == 0) return 0;  // mb_selective_scan says what is wrong
   Split sp;
   return split_layout(*a, nullptr, &sp);
 }

@@ -34,31 +34,44 @@ def _refuse(what):
 
 def _inputs(fn, x, **others):
     """x fixes device and type; every other tensor must be on x's device, none may need a gradient.  Returns the device index."""
+    try:
+        index = x.get_device()  # -1 on the host
+        good = index >= 0 and x.dtype in _DTYPES
+        grad = torch.is_grad_enabled()
+        wanted = grad and x.requires_grad
+        for t in others.values():
+            if t is not None:
+                good = good and t.get_device() == index
+                wanted = wanted or (grad and t.requires_grad)
+        if good and not wanted:
+            return index
+    except AttributeError:
+        pass
+    _refuse_inputs(fn, x, others)
+
+
+def _refuse_inputs(fn, x, others):
     if not torch.is_tensor(x) or x.dtype not in _DTYPES:
         _refuse(f"{fn}: x must be a float32, float16 or bfloat16 tensor, not {getattr(x, 'dtype', type(x).__name__)}")
     if not x.is_cuda:
         _refuse(f"{fn} needs CUDA(HIP) tensors; there is no CPU path")
-    grad = torch.is_grad_enabled()
-    if grad and x.requires_grad:
-        _refuse(f"{fn} has no backward: x requires grad (use torch.no_grad() or detach it)")
-    dev = x.device
     for name, t in others.items():
         if t is None:
             continue
         if not torch.is_tensor(t):
             _refuse(f"{fn}: {name} must be a tensor, not {type(t).__name__}")
-        if t.device != dev:
-            _refuse(f"{fn}: {name} is on {t.device}, x on {dev}")
-        if grad and t.requires_grad:
+        if t.device != x.device:
+            _refuse(f"{fn}: {name} is on {t.device}, x on {x.device}")
+    for name, t in dict(x=x, **others).items():
+        if t is not None and t.requires_grad:
             _refuse(f"{fn} has no backward: {name} requires grad (use torch.no_grad() or detach it)")
-    return dev.index
 
 
 def _param(fn, name, t, *shape):
     """fp32, contiguous, of that shape; None stays None."""
     if t is None:
         return None
-    if t.dtype is not torch.float32 or tuple(t.shape) != shape or not t.is_contiguous():
+    if t.dtype is not torch.float32 or t.shape != shape or not t.is_contiguous():
         _refuse(f"{fn}: {name} must be contiguous float32 {list(shape)}, got {t.dtype} {list(t.shape)} with strides {t.stride()}")
     return t.data_ptr()
 
@@ -76,9 +89,11 @@ def _rows(fn, name, t, lead, tail, dtype):
     """(batch stride, row stride) of a tensor of `lead` rows of `tail`, dense within a row."""
     if t.dtype is not dtype:
         _refuse(f"{fn}: {name} is {t.dtype}, expected {dtype}")
-    if tuple(t.shape) != lead + tail:
+    if t.shape != lead + tail:
         _refuse(f"{fn}: {name} has shape {list(t.shape)}, expected {list(lead + tail)}")
     st, dense = t.stride(), 1
+    if st[-1] == 1 and (len(tail) == 1 or (len(tail) == 2 and st[-2] == tail[1])):
+        return (st[0], st[1]) if len(lead) == 2 else (0, st[0])
     for i in range(len(tail)):
         if tail[-1 - i] != 1 and st[-1 - i] != dense and t.numel():
             _refuse(f"{fn}: {name} must be dense within a row of {list(tail)}; its strides are {st}")
@@ -89,46 +104,59 @@ def _rows(fn, name, t, lead, tail, dtype):
 
 def _extent(t):
     """Address range of a tensor, empty tensors have none."""
-    if t.numel() == 0:
+    n = t.numel()
+    if n == 0:
         return 0, 0
     lo = t.data_ptr()
-    return lo, lo + t.element_size() * (1 + sum((s - 1) * d for s, d in zip(t.shape, t.stride())))
+    if not t.is_contiguous():
+        n = 1
+        for size, stride in zip(t.shape, t.stride()):
+            n += (size - 1) * stride
+    return lo, lo + t.element_size() * n
 
 
-def _apart(fn, out, lead, row, **others):
-    """An output must not hold a row twice, nor overlap an input -- unless both are different columns of the same rows."""
-    strides = sorted((st, n) for st, n in zip(out.stride()[:len(lead)], lead) if n > 1)
-    need = row
-    for st, n in strides:
-        if st < need:
-            _refuse(f"{fn}: out's rows overlap each other (strides {out.stride()})")
-        need = st * (n - 1) + need
+def _apart(fn, out, lead, row, *others):
+    """An output must not hold a row twice, nor overlap an input ((name, tensor) pairs) -- unless both are different columns of the same
+    rows."""
+    if not out.is_contiguous():
+        need = row
+        for st, n in sorted((st, n) for st, n in zip(out.stride()[:len(lead)], lead) if n > 1):
+            if st < need:
+                _refuse(f"{fn}: out's rows overlap each other (strides {out.stride()})")
+            need = st * (n - 1) + need
     lo, hi = _extent(out)
-    for name, t in others.items():
+    for name, t in others:
         if t is None:
             continue
         a, b = _extent(t)
-        if lo >= b or a >= hi:
-            continue
-        k = len(lead)
-        same = t.element_size() == out.element_size() and tuple(t.shape[:k]) == lead and all(
-            n == 1 or p == q for n, p, q in zip(lead, t.stride(), out.stride()))
-        if same and strides:
-            step, e = strides[0][0] * out.element_size(), out.element_size()
-            width = t[(0,) * k].numel() * e
-            off = (a - lo) % step
-            if off >= row * e and off + width <= step:
-                continue
-        _refuse(f"{fn}: out overlaps {name}")
+        if lo < b and a < hi and not _other_columns(out, t, lead, row, a - lo):
+            _refuse(f"{fn}: out overlaps {name}")
+
+
+def _other_columns(out, t, lead, row, off):
+    """t, `off` bytes behind out, holds other columns of the same rows."""
+    k, e = len(lead), out.element_size()
+    strides = sorted(st for st, n in zip(out.stride(), lead) if n > 1)
+    if not strides or t.element_size() != e or tuple(t.shape[:k]) != lead or any(
+            n > 1 and p != q for n, p, q in zip(lead, t.stride(), out.stride())):
+        return False
+    step, width = strides[0] * e, t[(0,) * k].numel() * e
+    off %= step
+    return off >= row * e and off + width <= step
+
+
+_raw_stream = torch._C._cuda_getCurrentRawStream  # torch.cuda.current_stream(index).cuda_stream, without the object around it
 
 
 def _launch(fn, index, call, *args):
     """The call on the current stream of the tensors' device."""
     if index == torch.cuda.current_device():
-        _lib.check(call(*args, torch.cuda.current_stream().cuda_stream), fn)
+        rc = call(*args, _raw_stream(index))
     else:
         with torch.cuda.device(index):
-            _lib.check(call(*args, torch.cuda.current_stream().cuda_stream), fn)
+            rc = call(*args, _raw_stream(index))
+    if rc:
+        _lib.check(rc, fn)
 
 
 def _requests(fn, lead, cu_seqlens, lengths):
@@ -200,7 +228,7 @@ def causal_conv1d(x, weight, bias=None, activation=None, *, cu_seqlens=None, len
     if out is None:
         out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     else:
-        _apart(fn, out, lead, c, x=x, state=state)
+        _apart(fn, out, lead, c, ("x", x), ("state", state))
     yb, yr = _rows(fn, "out", out, lead, (c,), x.dtype)
     a = _lib.CausalConv1dArgs(x.data_ptr(), out.data_ptr(), w, _param(fn, "bias", bias, c), st, sl, has, cu, valid, xb, xr, yb, yr,
                               st_stride, _DTYPES[x.dtype], batch, t, c, k, _activation(fn, activation), n_slots)
@@ -223,7 +251,7 @@ def causal_conv1d_step(x, state, weight, bias=None, activation=None, *, slots=No
     if out is None:
         out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     else:
-        _apart(fn, out, (b,), c, x=x, state=state)
+        _apart(fn, out, (b,), c, ("x", x), ("state", state))
     _, yr = _rows(fn, "out", out, (b,), (c,), x.dtype)
     a = _lib.CausalConv1dArgs(x.data_ptr(), out.data_ptr(), w, _param(fn, "bias", bias, c), st, sl, None, None, None, 0, xr, 0, yr,
                               st_stride, _DTYPES[x.dtype], b, 1, c, k, _activation(fn, activation), n_slots)
@@ -262,7 +290,7 @@ def _scan_args(fn, step, x, dt, A, B, C_, D, dt_bias, dt_softplus, dt_limit, cu_
     if out is None:
         out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     else:
-        _apart(fn, out, lead, h * p, x=x, dt=dt, B=B, C=C_, state=state)
+        _apart(fn, out, lead, h * p, ("x", x), ("dt", dt), ("B", B), ("C", C_), ("state", state))
     yb, yr = _rows(fn, "out", out, lead, (h, p), x.dtype)
     if A is None:
         _refuse(f"{fn}: A is required")
@@ -304,6 +332,8 @@ def _row_stride(fn, name, t, shape, dtype):
     if t.shape != shape:
         _refuse(f"{fn}: {name} has shape {list(t.shape)}, expected {list(shape)}")
     st = t.stride()
+    if len(st) == 2 and st[1] == 1 and shape[0] > 1:
+        return st[0]
     if shape[-1] > 1 and st[-1] != 1:
         _refuse(f"{fn}: {name} must be dense within a row; its strides are {st}")
     step, rows = None, 1

@@ -84,9 +84,9 @@ def test_facade_checks_without_a_gpu(lib):
     assert ssm._rows("f", "t", rows[:, 2:6], (6,), (4,), torch.float32) == (0, 10)
     with pytest.raises(_lib.MbHipError, match="dense"):
         ssm._rows("f", "t", rows[:, ::2], (6,), (5,), torch.float32)
-    ssm._apart("f", rows[:, :4], (6,), 4, x=rows[:, 4:8])  # other columns of the same rows
+    ssm._apart("f", rows[:, :4], (6,), 4, ("x", rows[:, 4:8]))  # other columns of the same rows
     with pytest.raises(_lib.MbHipError, match="overlaps x"):
-        ssm._apart("f", rows[:, :4], (6,), 4, x=rows[:, 3:7])
+        ssm._apart("f", rows[:, :4], (6,), 4, ("x", rows[:, 3:7]))
     with pytest.raises(_lib.MbHipError, match="each other"):
         ssm._apart("f", rows[:1].expand(6, 10), (6,), 10)
     assert ssm._row_stride("f", "t", torch.zeros(2, 3, 8)[..., :5], torch.Size((2, 3, 5)), torch.float32) == 8
