@@ -113,7 +113,7 @@ __global__ __launch_bounds__(256) void causal_conv1d_kernel(const mb_causal_conv
 template <typename T, int K>
 __global__ __launch_bounds__(64) void causal_conv1d_step_kernel(const mb_causal_conv1d_args a) {
   constexpr bool FAST = sizeof(T) == 2;
-  constexpr int V = 8 / sizeof(T);
+  constexpr int V = CONV_V;
   const int per = (a.channels + 64 * V - 1) / (64 * V);
   const int b = (int)(blockIdx.x / per);
   const int c = ((int)(blockIdx.x - (unsigned)b * per) * 64 + (int)threadIdx.x) * V, n = a.channels - c;
@@ -125,10 +125,7 @@ __global__ __launch_bounds__(64) void causal_conv1d_step_kernel(const mb_causal_
 #pragma unroll
   for (int j = 0; j < K - 1; ++j) win[j] = load_some<T, V>(st + (long long)j * a.channels, n);
   float w[V][K];
-#pragma unroll
-  for (int i = 0; i < V; ++i)
-#pragma unroll
-    for (int j = 0; j < K; ++j) w[i][j] = i < n ? a.d_w[(long long)(c + i) * K + j] : 0.f;
+  load_taps<K, V>(a.d_w + (long long)c * K, n, w);
   const Vec<float, V> bias = load_some<float, V>(a.d_bias + c, a.d_bias ? n : 0);
 #pragma unroll
   for (int i = 0; i < V; ++i) {
@@ -147,7 +144,7 @@ __global__ __launch_bounds__(64) void causal_conv1d_step_kernel(const mb_causal_
 
 template <typename T, int K> int launch_conv(const mb_causal_conv1d_args& a, bool step, hipStream_t s) {
   if (step) {
-    const long long grid = (long long)a.batch * cdiv(a.channels, 64 * (8 / (int)sizeof(T)));
+    const long long grid = (long long)a.batch * cdiv(a.channels, 64 * CONV_V);
     MB_REQUIRE(grid < (1ll << 31), "causal_conv1d_step: %d items of %d channels are too many for one launch", a.batch, a.channels);
     hipLaunchKernelGGL((causal_conv1d_step_kernel<T, K>), dim3((unsigned)grid), dim3(64), 0, s, a);
   } else {

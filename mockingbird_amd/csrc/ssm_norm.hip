@@ -20,8 +20,12 @@ __device__ __forceinline__ float block_sum(float v, float* part, int waves) {  /
 }
 
 // One pass over memory: a row (or, where the first norm's groups are all that couples channels, one group of a row) is held in
-// registers, VPT vectors of 16 bytes per thread, by one wave (WAVE: no barrier, 4 rows per workgroup) or one workgroup.  Statistics are
-// two-pass (mean, then centred squares) in fp32.  Memory-bound: 4096 channels of bf16 move 6 bytes per element for a gated norm.
+// registers, VPT vectors of 16 bytes per thread, by one wave (WAVE: up to 64 vectors, no barrier, 4 rows per workgroup) or one workgroup.
+// Statistics are two-pass (mean, then centred squares) in fp32.  Memory-bound: 16384 x 4096 bf16 in 8 gated groups (6 bytes per element)
+// takes 79 us, 5.1 TB/s, a large copy's rate; 8192 x 2048 bf16 with an fp32 residual (12 bytes) 38 us, 5.3 TB/s.
+// Why these widths: a wave with 4 vectors per lane holds 162 registers and ran that second case in 46 us; one vector per thread in
+// workgroups of more than 256 threads loses to two (3001 fp16 channels: 46 and 41 us) unless there are too few rows to fill the chip
+// (64 rows of 4096: 6.2 and 7.6 us); four vectors of a 16-bit type spill at 1024 threads, so they begin where two end.
 template <typename T, typename TR, int VPT, bool WAVE>
 __global__ __launch_bounds__(WAVE ? 256 : 1024) void block_norm_kernel(const mb_block_norm_args a, int parts, long long units) {
   constexpr bool FAST = sizeof(T) == 2;
@@ -252,19 +256,15 @@ template <typename T, typename TR> int launch_norm(const mb_block_norm_args& a, 
   const int parts = a.next_norm ? 1 : a.groups, C = a.channels / parts, nv = cdiv(C, V);
   const long long units = a.rows * parts;
   const bool grouped = a.groups != parts;
-  // One wave per row up to 256 vectors; with few rows a wider row is dealt to a workgroup, whose loads are then in flight at once.
-  const bool wave = !grouped && nv <= 256 && (nv <= 64 || units >= 1024);
+  const bool wave = !grouped && nv <= 64;
   const bool whole = nv <= 4096 && (!grouped || (C / a.groups) % V == 0) && units < (1ll << 31);
   const size_t lds = whole && !wave && grouped ? ((size_t)nv + 2 * a.groups) * sizeof(float) : 0;
 #define MB_NORM(VPT, WAVE, GRID, THREADS) \
   hipLaunchKernelGGL((block_norm_kernel<T, TR, VPT, WAVE>), dim3((unsigned)(GRID)), dim3(THREADS), lds, s, a, parts, units)
   if (whole && wave) {
-    const long long grid = (units + 3) / 4;
-    if (nv <= 64) MB_NORM(1, true, grid, 256);
-    else if (nv <= 128) MB_NORM(2, true, grid, 256);
-    else MB_NORM(4, true, grid, 256);
+    MB_NORM(1, true, (units + 3) / 4, 256);
   } else if (whole) {
-    const int vpt = nv <= 512 ? 1 : nv <= 2048 ? 2 : 4, threads = (cdiv(nv, vpt) + 63) / 64 * 64;
+    const int vpt = nv <= (units < 512 ? 1024 : 256) ? 1 : nv <= 2048 ? 2 : 4, threads = (cdiv(nv, vpt) + 63) / 64 * 64;
     if (vpt == 1) MB_NORM(1, false, units, threads);
     else if (vpt == 2) MB_NORM(2, false, units, threads);
     else MB_NORM(4, false, units, threads);
