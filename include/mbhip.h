@@ -773,7 +773,8 @@ int mb_wave_finish_batch(const float* d_wav, const long long* d_pieces, int n_pi
  *    Rows: activations are time-major rows with a row stride (elements), dense within a row.  Two forms:
  *      packed   d_cu_seqlens != NULL: int32 [batch + 1], item b is the rows cu[b] .. cu[b+1]-1 of one [t] row axis (t = rows in all);
  *      padded   d_cu_seqlens == NULL: [batch][t] rows with a batch stride; item b is its first d_valid[b] rows (NULL: all t).
- *    Row numbers are read on the device: values outside 0..t are taken as 0 or t.  Rows that belong to no item are left as they were.
+ *    Row numbers are read on the device: values outside 0..t are taken as 0 or t (whatever they are, nothing outside the tensors is
+ *    touched; items must not share rows).  Rows that belong to no item are left as they were.
  *    State pools: [n_slots] states, item b owns slot d_slots[b] (NULL: slot b).  An item whose slot is outside 0..n_slots-1, or is named
  *    by an earlier item of the call too, is left out: neither its rows nor a state are written.  d_has_state[b] == 0: the item starts from
  *    zeros whatever its slot holds (NULL: every item continues).  A state is updated in place, also that of an item without rows.

@@ -192,7 +192,7 @@ static int check_conv(const char* name, const mb_causal_conv1d_args* a, bool ste
     MB_REQUIRE(!a->d_slots && !a->d_has_state, "%s: slots or has_state without a state pool", name);
   }
   MB_REQUIRE(!a->d_cu_seqlens || !a->d_valid, "%s: packed and padded rows at once", name);
-  MB_REQUIRE(!a->d_cu_seqlens || (long long)a->t + a->batch < (1ll << 31), "%s: %d rows of %d items are too many", name, a->t, a->batch);
+  MB_REQUIRE(step || (a->t <= 1 << 30 && a->batch <= 1 << 30), "%s: %d rows of %d items are too many", name, a->t, a->batch);
   return 1;
 }
 

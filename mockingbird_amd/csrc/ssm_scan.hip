@@ -83,7 +83,7 @@ __global__ __launch_bounds__(256) void selective_scan_join_kernel(const mb_selec
   const int parts = (rows_of(rows, b, first) + sp.seg - 1) / sp.seg;
   if (parts <= 1) return;  // not split: its workgroups read and write the pool themselves
   const long long tile = first_tile_of(rows, b, sp.seg);
-  if (n <= 0) return;
+  if (n <= 0 || tile + parts > sp.tiles) return;  // (row numbers that overlap can claim more tiles than there are)
   const bool keep = a.d_state && (!a.d_has_state || a.d_has_state[b]);
   Vec<float, 4> h = load_some<float, 4>(a.d_state + slot * a.state_stride + (long long)head * elems + e, keep ? n : 0);
   const long long step = (long long)a.heads * elems;
@@ -148,9 +148,11 @@ static int rows_per_tile(const mb_selective_scan_args& a) {
 static size_t split_layout(const mb_selective_scan_args& a, void* base, Split* sp) {
   sp->seg = rows_per_tile(a);
   sp->state = sp->decay = nullptr;
+  sp->tiles = 0;
   if (!sp->seg) return 0;
   const Rows rows = {a.d_cu_seqlens, a.d_valid, a.batch, a.t};
   const size_t tiles = (size_t)tiles_of(rows, sp->seg);
+  sp->tiles = (int)tiles;
   Arena ar(base, ~(size_t)0);
   sp->state = ar.take<float>(tiles * a.heads * a.head_dim * a.d_state_dim);
   sp->decay = ar.take<float>(tiles * a.heads);
@@ -179,7 +181,7 @@ static int check_scan(const char* name, const mb_selective_scan_args* a, bool st
     MB_REQUIRE(!a->d_slots && !a->d_has_state, "%s: slots or has_state without a state pool", name);
   }
   MB_REQUIRE(!a->d_cu_seqlens || !a->d_valid, "%s: packed and padded rows at once", name);
-  MB_REQUIRE(!a->d_cu_seqlens || (long long)a->t + a->batch < (1ll << 31), "%s: %d rows of %d items are too many", name, a->t, a->batch);
+  MB_REQUIRE(step || (a->t <= 1 << 30 && a->batch <= 1 << 30), "%s: %d rows of %d items are too many", name, a->t, a->batch);
   return 1;
 }
 

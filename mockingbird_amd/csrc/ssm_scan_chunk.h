@@ -219,6 +219,7 @@ struct Split {
   float* state;  // [tiles][heads][head_dim][d_state]
   float* decay;  // [tiles][heads]
   int seg;       // rows of a tile, a multiple of L; 0: not split
+  int tiles;     // that the workspace has room for
 };
 
 __device__ __forceinline__ float exp2_of(float v) { return __builtin_amdgcn_exp2f(v); }

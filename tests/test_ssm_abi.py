@@ -49,7 +49,7 @@ def norm(**kw):
     (conv, dict(dtype=2), "dtype"), (conv, dict(ksize=1), "ksize"), (conv, dict(ksize=9), "ksize"), (conv, dict(act=2), "act"), (conv, dict(batch=-1), "negative"),
     (conv, dict(d_w=None), "weight"), (conv, dict(d_x=None), "null"), (conv, dict(d_state=256, n_slots=1), "slots"), (conv, dict(d_slots=256), "pool"),
     (conv, dict(d_cu_seqlens=256, d_valid=256), "packed"), (conv, dict(batch=1 << 30, t=1 << 30), "too many"),
-    (conv, dict(d_cu_seqlens=256, t=(1 << 31) - 1), "too many"),
+    (conv, dict(d_cu_seqlens=256, t=(1 << 31) - 1), "too many"), (scan, dict(t=(1 << 30) + 1), "too many"),
     (scan, dict(dtype=2), "dtype"), (scan, dict(dt_dtype=1), "dt_dtype"), (scan, dict(head_dim=0), "head_dim"), (scan, dict(head_dim=129), "head_dim"),
     (scan, dict(d_state_dim=257), "d_state"), (scan, dict(groups=3), "groups"), (scan, dict(dt_min=2.0), "dt_min"), (scan, dict(dt_min=float("nan")), "dt_min"),
     (scan, dict(d_a=None), "no A"), (scan, dict(d_c=None), "null"), (scan, dict(d_has_state=256), "pool"), (scan, dict(batch=1 << 30, heads=4, t=1 << 30), "too many"),

@@ -542,6 +542,153 @@ def test_offsets_beyond_32_bits():
         assert torch.equal(got, want)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", [(2, 64, 64, 1), (4, 128, 128, 2), (2, 64, 256, 1), (6, 64, 128, 1)])
+def test_selective_scan_of_whole_tiles(dtype, shape):
+    """Head sizes without partial tiles (buffer accesses), over several chunks, split along time, in packed slices and padded batches."""
+    from mockingbird_amd import ssm
+    h, p, n, g = shape
+    for packed, lens in [(True, [700, 0, 1, 333]), (False, [500, 64, 301])]:
+        r = gen(h * n + packed)
+        args, lead, t = meta(lens, packed)
+        x, dt, a, bm, cm, skip, bias = scan_inputs(r, lead, h, p, n, g, dtype)
+        a = a * 0.2
+        seqs = ref.sequences(lens, packed, t)
+        pool, slots, has = pool_of(len(lens), (h, p, n), seqs, r, F32)
+        dpool = pool.cuda()
+        row = torch.cat([x.flatten(-2), bm.flatten(-2), cm.flatten(-2)], -1).cuda()  # one projection's output
+        d = h * p
+        out = torch.full(x.shape, 7.0, dtype=dtype, device="cuda")
+        y = ssm.selective_scan(row[..., :d].unflatten(-1, (h, p)), dt.cuda(), a.cuda(), row[..., d:d + g * n].unflatten(-1, (g, n)),
+                               row[..., d + g * n:].unflatten(-1, (g, n)), skip.cuda(), dt_bias=bias.cuda(), dt_softplus=True, state=dpool, out=out,
+                               **args, **slot_args(slots, has))
+        want, err, new, nerr = ref.scan(flat(x, 2), flat(dt, 1), a, flat(bm, 2), flat(cm, 2), skip, bias, True, None, seqs, pool, slots, has,
+                                        PLANES[dtype])
+        got = y.reshape(-1, h, p).cpu()
+        rows = torch.isnan(want)[:, 0, 0]
+        assert (got[rows] == 7.0).all(), "rows of no item were written"
+        ref.check(got[~rows], want[~rows], ref.rounded(want, err, dtype)[~rows], (lens, "y"))
+        ref.check(dpool.cpu()[slots], new[slots], nerr[slots] + ref.HALF[F32] * new[slots].abs() + ref.TINY[F32], (lens, "state"))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("value", [NAN, float("-inf")])
+def test_selective_scan_of_whole_tiles_stays_causal(dtype, value):
+    """The same around a NaN or infinity in one column of one head: nothing before it, no other column and no other head changes."""
+    from mockingbird_amd import ssm
+    h, p, n, t = 2, 64, 64, 150
+    r = gen(8)
+    x, dt, a, bm, cm, skip, bias = scan_inputs(r, (t,), h, p, n, 1, dtype)
+    clean = x.clone()
+    for row, head, col in [(37, 0, 5), (100, 1, 60)]:
+        x[row, head, col] = value
+    y = ssm.selective_scan(x.cuda(), dt.cuda(), a.cuda(), bm.cuda(), cm.cuda(), skip.cuda(), dt_bias=bias.cuda(), dt_softplus=True, cu_seqlens=i32(0, t)).cpu()
+    want, err, _, _ = ref.scan(clean, dt, a, bm, cm, skip, bias, True, None, [(0, t)], planes=PLANES[dtype])
+    bound = ref.rounded(want, err, dtype)
+    hit = torch.zeros(t, h, p, dtype=torch.bool)
+    hit[37:, 0, 5] = True
+    hit[100:, 1, 60] = True
+    assert not torch.isfinite(y[hit]).any()
+    ref.check(y[~hit], want[~hit], bound[~hit])
+
+
+def test_a_split_prompt_in_a_graph():
+    """The two passes of a long prompt captured, replayed on new inputs between eager calls, in two graphs with pools of their own."""
+    from mockingbird_amd import ssm
+    h, p, n, t = 2, 64, 64, 900
+    x, dt, a, bm, cm, skip, bias = [v.cuda() for v in scan_inputs(gen(1), (t,), h, p, n, 1, BF16)]
+    cu, pool0 = i32(0, 600, t), torch.randn(2, h, p, n, device="cuda")
+
+    def call(pool):
+        return ssm.selective_scan(x, dt, a, bm, cm, skip, dt_bias=bias, dt_softplus=True, cu_seqlens=cu, state=pool)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call(pool0.clone())
+    torch.cuda.current_stream().wait_stream(side)
+    graphs = []
+    for _ in range(2):
+        pool = pool0.clone()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            y = call(pool)
+        graphs.append((g, pool, y))
+    for i in range(3):
+        x.copy_(gen(30 + i)(t, h, p, dtype=BF16))
+        want_pool = pool0.clone()
+        want = call(want_pool)
+        for g, pool, y in graphs:
+            pool.copy_(pool0)
+            g.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(y, want) and torch.equal(pool, want_pool)
+
+
+def test_row_numbers_that_overlap_touch_nothing_else():
+    """Items that claim the same rows (which is not allowed) still write only rows and slots of their own tensors."""
+    from mockingbird_amd import ssm
+    h, p, n, t = 2, 32, 16, 700
+    x, dt, a, bm, cm, skip, bias = [v.cuda() for v in scan_inputs(gen(2), (t,), h, p, n, 1, F32)]
+    cu = i32(*([0, t] * 6), 0)
+    wide = torch.full((t + 64, h, p), 7.0, device="cuda")
+    pools = torch.full((14, h, p, n), 3.0, device="cuda")
+    ssm.selective_scan(x, dt, a, bm, cm, skip, dt_bias=bias, dt_softplus=True, cu_seqlens=cu, state=pools[1:13], out=wide[:t])
+    cx = torch.full((t + 64, 48), 7.0, device="cuda")
+    ssm.causal_conv1d(torch.zeros(t, 48, device="cuda"), torch.zeros(48, 4, device="cuda"), cu_seqlens=cu, out=cx[:t])
+    torch.cuda.synchronize()
+    assert (wide[t:] == 7.0).all() and (cx[t:] == 7.0).all() and (pools[[0, 13]] == 3.0).all()
+
+
+def test_many_items():
+    """More items than a wave sums up at once, most of them short, some empty."""
+    from mockingbird_amd import ssm
+    lens = [(7 * i) % 11 for i in range(150)] + [300] + [i % 3 for i in range(60)]
+    args, lead, t = meta(lens, True)
+    h, p, n = 2, 16, 16
+    r = gen(3)
+    x, dt, a, bm, cm, skip, bias = scan_inputs(r, lead, h, p, n, 1, BF16)
+    pool, slots, has = pool_of(len(lens), (h, p, n), lens, r, F32)
+    dpool = pool.cuda()
+    y = ssm.selective_scan(x.cuda(), dt.cuda(), a.cuda(), bm.cuda(), cm.cuda(), skip.cuda(), dt_bias=bias.cuda(), dt_softplus=True, state=dpool,
+                           **args, **slot_args(slots, has))
+    seqs = ref.sequences(lens, True, t)
+    want, err, new, nerr = ref.scan(x, dt, a, bm, cm, skip, bias, True, None, seqs, pool, slots, has, PLANES[BF16])
+    ref.check(y, want, ref.rounded(want, err, BF16))
+    ref.check(dpool.cpu()[slots], new[slots], nerr[slots] + ref.HALF[F32] * new[slots].abs() + ref.TINY[F32])
+    cx, w = r(*lead, 40, dtype=BF16), r(40, 4)
+    cpool, slots, has = pool_of(len(lens), (3, 40), lens, r, BF16)
+    dc = cpool.cuda()
+    y = ssm.causal_conv1d(cx.cuda(), w.cuda(), state=dc, **args, **slot_args(slots, has))
+    want, err, new = ref.conv(cx, w, None, None, seqs, cpool, slots, has)
+    ref.check(y, want, ref.rounded(want, err, BF16))
+    assert torch.equal(dc.cpu()[slots].double(), new[slots])
+
+
+def test_two_streams_at_once():
+    """Calls on two streams share nothing: each gives what it gives alone."""
+    from mockingbird_amd import ssm
+    h, p, n, t = 2, 64, 64, 1200
+    ins = [[v.cuda() for v in scan_inputs(gen(40 + i), (t,), h, p, n, 1, BF16)] for i in range(2)]
+    cu = i32(0, t)
+
+    def call(v):
+        x, dt, a, bm, cm, skip, bias = v
+        return ssm.selective_scan(x, dt, a, bm, cm, skip, dt_bias=bias, dt_softplus=True, cu_seqlens=cu)
+
+    alone = [call(v) for v in ins]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(5):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(call(ins[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(y, alone[i]) for y in got[i])
+
+
 # ---------------------------------------------------------------------------------------------- refusals
 
 def refusals():
