@@ -3,7 +3,7 @@
 //   h   <- exp(s(L)) h + sum_s exp(s(L) - s(s)) d_s x_s B_s^T
 // i.e. four products per chunk and head: G = C B^T (shared by the heads of a group), M x, C h, and x^T B.
 //
-// A workgroup takes two heads of one group and 64 of their columns (two waves per head, 32 columns each) and walks along time; h stays
+// A workgroup takes two heads of one group and 64 of their columns (four waves per head, 16 columns each) and walks along time; h stays
 // in the accumulators (fp32) of those waves for the whole walk and never visits LDS or memory between chunks.  Every product is written
 // so that one factor is already in the register layout the matrix instruction wants: in the accumulators of two stacked 16x16x32 tiles a
 // lane holds rows 4 g + i of both (g = lane >> 4) of column lane & 15, which is an operand whose inner index is dealt out as those rows.
@@ -11,9 +11,14 @@
 // order: x^T by transposing reads of rows 4 g + i and 16 + 4 g + i; for C h the state's rows are numbered so that the order is C's own
 // (tile 2 q holds columns 32 q + 8 g + i, tile 2 q + 1 those 4 further on).
 //
-// Two workgroups fit a CU: while one waits at a barrier or converts operands, the other's products run.  What bounds it is the vector
-// pipe (splitting h, M and c x into planes), not the matrix pipe; hence M is formed once per head and goes through LDS, and B, C are
-// shared by two heads only.
+// What bounds it is the vector pipe, which splits h, M and c x into planes (about 560 instructions per wave and chunk beside 91 matrix
+// instructions), and the order of a chunk: step sizes, G, M, M x.  Hence: M is formed once per head and goes through LDS; two
+// workgroups of 8 waves fit a CU (78 KB of LDS, 128 registers, nothing spilled -- a reload waits for the loads in flight in front of it),
+// so that one's products run while the other waits; the terms of the step sizes are a chunk ahead; the conversion of the next operand
+// stands between the products of this one.  Four waves of 32 columns read LDS half as often and are no faster (8192 rows, 64 heads of
+// 64 x 128: 149 and 146 us), one workgroup of four heads neither.
+// Measured, 8192 rows x 64 heads of 64 columns, 128 states, bf16: 80 us this pass, 41 us the states' pass, 13 us the join between them, of
+// 28 us that its bytes take at a large copy's rate.  Planes less would save 9 us (h and M in one) and 10 us (c x in two) of it.
 //
 // Precision.  Every sum, the state and all exponents are fp32 (prefix sums over a chunk: fp64, so that differences of far rows keep
 // their bits).  Operands are bf16 planes: a raw value is exact in 1 (bf16), 2 (fp16) or 3 (fp32) planes; computed operands are split as
@@ -30,7 +35,7 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
-// exp and the step sizes are the library's fp32 functions: a decay error of one step is taken to the power of the sequence's length
+// Step sizes and decays keep fp32's full accuracy whatever the activations' type: a decay's error is taken to the power of the rows it spans.
 __device__ __forceinline__ float step_raw(const mb_selective_scan_args& a, long long at) {
   return a.dt_dtype == MB_F32 ? ((const float*)a.d_dt)[at] : a.dt_dtype == MB_F16 ? to_f32(((const f16*)a.d_dt)[at]) : to_f32(((const bf16*)a.d_dt)[at]);
 }
