@@ -226,7 +226,7 @@ def causal_conv1d(x, weight, bias=None, activation=None, *, cu_seqlens=None, len
     w, k = _conv_weight(fn, weight, c)
     st, st_stride, n_slots, sl, has = _pool(fn, state, x.dtype, (k - 1, c), batch, slots, has_state)
     if out is None:
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        out = x.new_empty(lead + (c,))
     else:
         _apart(fn, out, lead, c, ("x", x), ("state", state))
     yb, yr = _rows(fn, "out", out, lead, (c,), x.dtype)
@@ -249,7 +249,7 @@ def causal_conv1d_step(x, state, weight, bias=None, activation=None, *, slots=No
     w, k = _conv_weight(fn, weight, c)
     st, st_stride, n_slots, sl, _ = _pool(fn, state, x.dtype, (k - 1, c), b, slots, None)
     if out is None:
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        out = x.new_empty((b, c))
     else:
         _apart(fn, out, (b,), c, ("x", x), ("state", state))
     _, yr = _rows(fn, "out", out, (b,), (c,), x.dtype)
@@ -288,7 +288,7 @@ def _scan_args(fn, step, x, dt, A, B, C_, D, dt_bias, dt_softplus, dt_limit, cu_
     cb, cr = _rows(fn, "C", C_, lead, (g, n), x.dtype)
     st, st_stride, n_slots, sl, has = _pool(fn, state, torch.float32, (h, p, n), batch, slots, has_state)
     if out is None:
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        out = x.new_empty(lead + (h, p))
     else:
         _apart(fn, out, lead, h * p, ("x", x), ("dt", dt), ("B", B), ("C", C_), ("state", state))
     yb, yr = _rows(fn, "out", out, lead, (h, p), x.dtype)
@@ -311,7 +311,7 @@ def selective_scan(x, dt, A, B, C, D=None, *, dt_bias=None, dt_softplus=False, d
                                out)
     lib = _lib.lib()
     need = lib.mb_selective_scan_workspace_bytes(a)
-    ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
+    ws = x.new_empty((need,), dtype=torch.uint8) if need else None
     _launch(fn, index, lib.mb_selective_scan, a, _lib.ptr(ws), need)
     return out
 
@@ -409,7 +409,7 @@ def block_norm(x, weight=None, bias=None, *, norm="rms", eps=1e-5, groups=1, gat
         total, y = residual_out, out
     rows = x.numel() // c if c else 0
     if total is None:
-        total, ss = torch.empty(shape, dtype=sum_dtype, device=x.device), c
+        total, ss = x.new_empty(tuple(shape), dtype=sum_dtype), c
     else:
         ss = _row_stride(fn, "residual_out" if next_norm or residual_out is not None else "out", total, shape, sum_dtype)
         if rows > 1 and ss < c:
@@ -418,7 +418,7 @@ def block_norm(x, weight=None, bias=None, *, norm="rms", eps=1e-5, groups=1, gat
     ys = 0
     if next_norm is not None:
         if y is None:
-            y, ys = torch.empty(shape, dtype=x.dtype, device=x.device), c
+            y, ys = x.new_empty(tuple(shape)), c
         else:
             ys = _row_stride(fn, "out", y, shape, x.dtype)
             if rows > 1 and ys < c:
