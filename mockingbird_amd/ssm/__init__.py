@@ -26,6 +26,7 @@ _DTYPES = {torch.float32: _lib.MB_F32, torch.float16: _lib.MB_F16, torch.bfloat1
 _NORMS = {None: 0, "rms": 1, "layer": 2}
 _GATES = {None: 0, "silu": 1, "sigmoid": 2}
 _INF = float("inf")
+_F32 = torch.float32
 
 
 def _refuse(what):
@@ -71,9 +72,9 @@ def _param(fn, name, t, *shape):
     """fp32, contiguous, of that shape; None stays None."""
     if t is None:
         return None
-    if t.dtype is not torch.float32 or t.shape != shape or not t.is_contiguous():
-        _refuse(f"{fn}: {name} must be contiguous float32 {list(shape)}, got {t.dtype} {list(t.shape)} with strides {t.stride()}")
-    return t.data_ptr()
+    if t.dtype is _F32 and t.shape == shape and t.is_contiguous():
+        return t.data_ptr()
+    _refuse(f"{fn}: {name} must be contiguous float32 {list(shape)}, got {t.dtype} {list(t.shape)} with strides {t.stride()}")
 
 
 def _numbers(fn, name, t, dtype, n):
@@ -87,13 +88,14 @@ def _numbers(fn, name, t, dtype, n):
 
 def _rows(fn, name, t, lead, tail, dtype):
     """(batch stride, row stride) of a tensor of `lead` rows of `tail`, dense within a row."""
+    st = t.stride()
+    if t.dtype is dtype and t.shape == lead + tail and st[-1] == 1 and (len(tail) == 1 or (len(tail) == 2 and st[-2] == tail[1])):
+        return (st[0], st[1]) if len(lead) == 2 else (0, st[0])
     if t.dtype is not dtype:
         _refuse(f"{fn}: {name} is {t.dtype}, expected {dtype}")
     if t.shape != lead + tail:
         _refuse(f"{fn}: {name} has shape {list(t.shape)}, expected {list(lead + tail)}")
-    st, dense = t.stride(), 1
-    if st[-1] == 1 and (len(tail) == 1 or (len(tail) == 2 and st[-2] == tail[1])):
-        return (st[0], st[1]) if len(lead) == 2 else (0, st[0])
+    dense = 1
     for i in range(len(tail)):
         if tail[-1 - i] != 1 and st[-1 - i] != dense and t.numel():
             _refuse(f"{fn}: {name} must be dense within a row of {list(tail)}; its strides are {st}")
@@ -197,6 +199,8 @@ def _pool(fn, state, dtype, inner, batch, slots, has_state):
 
 
 def _conv_weight(fn, weight, channels):
+    if weight is None:
+        _refuse(f"{fn}: weight is required")
     if weight.dim() == 3 and weight.shape[1] == 1:  # torch's depthwise layout [channels, 1, taps]
         weight = weight[:, 0]
     if weight.dim() != 2 or not 2 <= weight.shape[1] <= 8:
@@ -262,6 +266,9 @@ def causal_conv1d_step(x, state, weight, bias=None, activation=None, *, slots=No
 def _scan_args(fn, step, x, dt, A, B, C_, D, dt_bias, dt_softplus, dt_limit, cu_seqlens, lengths, state, slots, has_state, out):
     index = _inputs(fn, x, dt=dt, A=A, B=B, C=C_, D=D, dt_bias=dt_bias, cu_seqlens=cu_seqlens, lengths=lengths, state=state, slots=slots,
                     has_state=has_state, out=out)
+    for name, t in (("dt", dt), ("A", A), ("B", B), ("C", C_)):
+        if t is None:
+            _refuse(f"{fn}: {name} is required")
     if x.dim() != 3 and (step or x.dim() != 4):
         _refuse(f"{fn}: x must be {'[batch, heads, head_dim]' if step else '[rows, heads, head_dim] or [batch, t, heads, head_dim]'}, "
                 f"got {list(x.shape)}")
@@ -292,8 +299,6 @@ def _scan_args(fn, step, x, dt, A, B, C_, D, dt_bias, dt_softplus, dt_limit, cu_
     else:
         _apart(fn, out, lead, h * p, ("x", x), ("dt", dt), ("B", B), ("C", C_), ("state", state))
     yb, yr = _rows(fn, "out", out, lead, (h, p), x.dtype)
-    if A is None:
-        _refuse(f"{fn}: A is required")
     a = _lib.SelectiveScanArgs(x.data_ptr(), out.data_ptr(), dt.data_ptr(), B.data_ptr(), C_.data_ptr(), _param(fn, "A", A, h),
                                _param(fn, "D", D, h), _param(fn, "dt_bias", dt_bias, h), st, sl, has, cu, valid, xb, xr, yb, yr, db, dr,
                                bb, br, cb, cr, st_stride, _DTYPES[x.dtype], _DTYPES[dt.dtype], batch, t, h, p, g, n, n_slots,

@@ -754,6 +754,15 @@ def test_refusals_of_steps_and_devices():
         ssm.causal_conv1d(x, w.cpu(), cu_seqlens=i32(0, 3))
     with pytest.raises(_lib.MbHipError, match="no CPU path"):
         ssm.block_norm(x.cpu())
+    with pytest.raises(_lib.MbHipError, match="weight is required"):
+        ssm.causal_conv1d(x, None, cu_seqlens=i32(0, 3))
+    s = torch.zeros(3, 2, 8, device="cuda")
+    with pytest.raises(_lib.MbHipError, match="B is required"):
+        ssm.selective_scan(s, s[..., 0].contiguous(), torch.zeros(2, device="cuda"), None, None, cu_seqlens=i32(0, 3))
+    with pytest.raises(_lib.MbHipError, match="dt has shape"):
+        ssm.selective_scan(s, torch.zeros((), device="cuda"), torch.zeros(2, device="cuda"), s[:, :1], s[:, :1], cu_seqlens=i32(0, 3))
+    with pytest.raises(_lib.MbHipError, match="must be a tensor"):
+        ssm.causal_conv1d(x, [1.0], cu_seqlens=i32(0, 3))
     p = torch.zeros(16, device="cuda", requires_grad=True)
     with pytest.raises(_lib.MbHipError, match="backward"):
         ssm.block_norm(x, p)
