@@ -135,7 +135,9 @@ static int rows_per_tile(const mb_selective_scan_args& a) {
   const long long units = (long long)a.groups * cdiv(a.heads / a.groups, 2) * cdiv(a.head_dim, 64);
   const long long all = a.d_cu_seqlens ? a.t : (long long)a.t * a.batch;
   const bool full = units * a.batch >= 256;
-  if (full && !a.d_cu_seqlens) return 0;
+  // up to five chunks one walk is shorter than three launches (24 heads of 64 x 128 bf16: 256 rows 28 and 33 us, 384 rows 37 and 33 us)
+  const int chunk = a.dtype == MB_BF16 && a.d_state_dim <= 128 ? 64 : 32;
+  if ((full && !a.d_cu_seqlens) || a.t <= 5 * chunk) return 0;
   long long seg = (all * units + 511) / 512;  // two workgroups per CU
   // shorter tiles shorten the walk but move more states: not below 128 rows where a head's state outweighs 64 rows of its x
   const int least = a.head_dim * a.d_state_dim < 4096 ? 64 : 128;
