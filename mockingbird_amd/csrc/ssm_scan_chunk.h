@@ -114,6 +114,20 @@ __device__ __forceinline__ f32x4 mma(const bf16x8 (&a)[QA], const bf16x8 (&b)[QB
   return acc;
 }
 
+// the same with the first 16 of a's 32 rows
+template <int QA, int QB, int K>
+__device__ __forceinline__ f32x4 mma_half(const bf16x8 (&a)[QA], const bf16x4 (&b)[QB], f32x4 acc) {
+#pragma unroll
+  for (int i = QA - 1; i >= 0; --i)
+#pragma unroll
+    for (int j = QB - 1; j >= 0; --j)
+      if (i + j < K) {
+        const bf16x4 lo = {a[i][0], a[i][1], a[i][2], a[i][3]};
+        acc = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(s16x4, lo), __builtin_bit_cast(s16x4, b[j]), acc, 0, 0, 0);
+      }
+  return acc;
+}
+
 template <typename T, int NP, bool STATES> struct ScanShape {
   static constexpr int R = sizeof(T) == 4 ? 3 : std::is_same<T, f16>::value ? 2 : 1;  // raw planes
   static constexpr int Q = R == 3 ? 3 : 2;                                             // planes of M and h
@@ -128,13 +142,20 @@ template <typename T, int NP, bool STATES> struct ScanShape {
   // LDS rows of B and C are 32 bytes longer than their data: 8 rows of one 16-byte unit lie in different banks.  x has no room for that (two
   // workgroups would not fit): its 32-byte pieces change places with the row, so that 4 rows of one piece do.
   static constexpr int NS = NP + 16;                       // row stride in halves
-  static __device__ __forceinline__ int x_col(int r, int c) { return c ^ 16 * (r >> 1 & 1); }
+  static __device__ __forceinline__ unsigned x_col(unsigned r, unsigned c) { return c ^ 16 * (r >> 1 & 1); }
   static constexpr int GT = TT * (TT + 1) / 2;             // causal tiles of G
   struct alignas(16) Head { float u[L], w[L], hi[L], lo[L], d[L], f[TT][TT], front[TT], back[TT], total; };
   // Step-size terms of HEADS chunks.  The states' pass, which needs no C and no M, has room for 8: every wave of a head does one of the next
   // four chunks at a time.  The other pass keeps this chunk's and the next one's, which one wave of each head does.
   static constexpr int HEADS = STATES ? 2 * WPH : 2;
-  struct LdsY { unsigned short c[R][L][NS]; bf16x4 m[HB][GT][Q][64]; };
+  struct LdsY { unsigned short c[R][L][NS]; bf16x4 m[HB][GT * Q * 64]; };
+  // Two s tiles of M^T next to each other are one operand of 32 rows (16 bytes a lane); the diagonal tiles of even rows of tiles have no
+  // partner and come first.  -> index of tile (i, j), plane q, this lane
+  static __device__ __forceinline__ int m_at(int i, int j, int q, int lane) {
+    if (i == j && i % 2 == 0) return (j / 2 * Q + q) * 64 + lane;
+    return TT / 2 * Q * 64 + 2 * ((pairs_before(j) + i / 2) * Q + q) * 64 + 2 * lane + i % 2;
+  }
+  static __device__ __forceinline__ int pairs_before(int j) { return (j / 2) * (j / 2) + (j % 2) * (j / 2); }  // in rows of tiles 0 .. j - 1
   struct LdsStates { double walked[HB][WPH]; };
   struct Lds : std::conditional<STATES, LdsStates, LdsY>::type {
     unsigned short b[R][L][NS], x[HB][R][L][PB];
@@ -180,8 +201,8 @@ template <typename T, int V, int ROWS, int COLS, int THREADS> struct Stage {
   }
   // The same where every column exists: through a buffer descriptor that ends behind row `rows` - 1, whose range check supplies the zeros.
   // One address register for all; the thread's further vectors are a fixed number of rows on.
-  static __device__ __forceinline__ unsigned offset(int tid, int rstride) {
-    return (unsigned)((tid / PER_ROW * rstride + tid % PER_ROW * V) * (int)sizeof(T));
+  static __device__ __forceinline__ unsigned offset(unsigned tid, int rstride) {
+    return (tid / PER_ROW * (unsigned)rstride + tid % PER_ROW * V) * (unsigned)sizeof(T);
   }
   __device__ __forceinline__ void request(const T* base, int rstride, int rows, unsigned off, int width) {
     // (31 bits hold it: the host looked)
@@ -191,10 +212,10 @@ template <typename T, int V, int ROWS, int COLS, int THREADS> struct Stage {
       v[i] = __builtin_bit_cast(Vec<T, V>, __builtin_amdgcn_raw_buffer_load_b128(d, off, i * (THREADS / PER_ROW) * rstride * (int)sizeof(T), 0));
   }
   // put(plane, row, column, V halves)
-  template <int R, typename F> __device__ __forceinline__ void lay(int tid, F put) {
+  template <int R, typename F> __device__ __forceinline__ void lay(unsigned tid, F put) {
 #pragma unroll
     for (int i = 0; i < COUNT; ++i) {
-      const int at = tid + i * THREADS, r = at / PER_ROW, c = at % PER_ROW * V;
+      const unsigned at = tid + i * THREADS, r = at / PER_ROW, c = at % PER_ROW * V;
       if (TOTAL % THREADS != 0 && r >= ROWS) continue;
       if constexpr (R == 1) {
         put(0, r, c, __builtin_bit_cast(Vec<unsigned short, V>, v[i]));
@@ -301,7 +322,7 @@ __global__ __launch_bounds__((ScanShape<T, NP, STATES>::THREADS), (ScanShape<T, 
 
   Stage<T, V, L, NP, THREADS> sb, sc;
   Stage<T, V, L, HB * PB, THREADS> sx;
-  auto request = [&](int t, int tid) {  // behind the last row: zeros without a load, so that no register has to keep an older chunk's values
+  auto request = [&](int t, unsigned tid) {  // behind the last row: zeros without a load, so that no register has to keep an older chunk's values
     const int n = t1 - t;
     if constexpr (WHOLE) {
       sb.request(bg + t * a.b_rstride, (int)a.b_rstride, min(n, L), sb.offset(tid, (int)a.b_rstride), NP);
@@ -323,10 +344,10 @@ __global__ __launch_bounds__((ScanShape<T, NP, STATES>::THREADS), (ScanShape<T, 
       });
     }
   };
-  auto lay = [&](int tid) {
-    sb.template lay<R>(tid, [&](int q, int r, int c, const Vec<unsigned short, V>& v) { store_lds<V>(&m.b[q][r][c], v); });
-    if constexpr (!STATES) sc.template lay<R>(tid, [&](int q, int r, int c, const Vec<unsigned short, V>& v) { store_lds<V>(&m.c[q][r][c], v); });
-    sx.template lay<R>(tid, [&](int q, int r, int c, const Vec<unsigned short, V>& v) { store_lds<V>(&m.x[c / PB][q][r][S::x_col(r, c % PB)], v); });
+  auto lay = [&](unsigned tid) {
+    sb.template lay<R>(tid, [&](int q, unsigned r, unsigned c, const Vec<unsigned short, V>& v) { store_lds<V>(&m.b[q][r][c], v); });
+    if constexpr (!STATES) sc.template lay<R>(tid, [&](int q, unsigned r, unsigned c, const Vec<unsigned short, V>& v) { store_lds<V>(&m.c[q][r][c], v); });
+    sx.template lay<R>(tid, [&](int q, unsigned r, unsigned c, const Vec<unsigned short, V>& v) { store_lds<V>(&m.x[c / PB][q][r][S::x_col(r, c % PB)], v); });
   };
   // scalars of the heads, read once: inside the loop they would be loads behind its stores
   auto scalar = [&](const float* p, int at) { return __uint_as_float(__builtin_amdgcn_readfirstlane(p ? __float_as_uint(p[at]) : 0u)); };
@@ -387,7 +408,7 @@ __global__ __launch_bounds__((ScanShape<T, NP, STATES>::THREADS), (ScanShape<T, 
       for (int j = 0; j < TT; ++j) walked += sum[j];
   };
 
-  if (WHOLE) request(t0, (int)threadIdx.x);
+  if (WHOLE) request(t0, threadIdx.x);
   constexpr int HEADS = S::HEADS, FOUR = S::WPH;
   const bool stepper = mine && quarter == FOUR - 1;  // the wave of each head that does this, a chunk ahead of the others' products
   if (STATES ? mine : stepper) {
@@ -403,7 +424,8 @@ __global__ __launch_bounds__((ScanShape<T, NP, STATES>::THREADS), (ScanShape<T, 
     // that are not there.
     int fresh = lane;
     asm volatile("" : "+v"(fresh));
-    const int g = fresh >> 4, li = fresh & 15, lane = fresh, tid = wave * 64 + fresh;
+    const int g = fresh >> 4, li = fresh & 15, lane = fresh;
+    const unsigned tid = (unsigned)(wave * 64 + fresh);
     if (!WHOLE) request(t, tid);  // masks and addresses of partial columns leave no registers to hold values through the products
     lay(tid);
     meet();
@@ -424,7 +446,7 @@ __global__ __launch_bounds__((ScanShape<T, NP, STATES>::THREADS), (ScanShape<T, 
       // TT waves, the others to the first 6 (the last two have the step sizes)
       constexpr int OFF = TT * (TT - 1) / 2;
       for (int k = wave < TT ? -1 : wave; k < OFF; k = k < 0 && wave < OFF ? wave : OFF) {
-        const int j = k < 0 ? wave : k < 1 ? 1 : k < 3 ? 2 : 3, i = k < 0 ? wave : k - j * (j - 1) / 2, at = j * (j + 1) / 2 + i;
+        const int j = k < 0 ? wave : k < 1 ? 1 : k < 3 ? 2 : 3, i = k < 0 ? wave : k - j * (j - 1) / 2;
         f32x4 gt = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int n = 0; n < NP; n += 32) {
@@ -464,7 +486,7 @@ __global__ __launch_bounds__((ScanShape<T, NP, STATES>::THREADS), (ScanShape<T, 
           for (int q = 0; q < Q; ++q) {
             typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
             const u32x2 w = {pack_bf16(x0, x1), pack_bf16(x2, x3)};
-            m.m[e][at][q][lane] = __builtin_bit_cast(bf16x4, w);
+            m.m[e][S::m_at(i, j, q, lane)] = __builtin_bit_cast(bf16x4, w);
             x0 -= __uint_as_float(w[0] << 16), x1 -= __uint_as_float(w[0] & 0xffff0000u);
             x2 -= __uint_as_float(w[1] << 16), x3 -= __uint_as_float(w[1] & 0xffff0000u);
           }
@@ -587,17 +609,17 @@ __global__ __launch_bounds__((ScanShape<T, NP, STATES>::THREADS), (ScanShape<T, 
 #pragma unroll
         for (int j = 0; j < TT; ++j) {
 #pragma unroll
-          for (int k = 0; k <= j / 2; ++k) {
+          for (int k = 0; 2 * k < j; ++k) {
             bf16x8 fm[Q];
 #pragma unroll
-            for (int q = 0; q < Q; ++q) {
-              const int at = j * (j + 1) / 2 + 2 * k;
-              const bf16x4 lo = m.m[hh][at][q][lane];
-              bf16x4 hi = {(__bf16)0.f, (__bf16)0.f, (__bf16)0.f, (__bf16)0.f};
-              if (2 * k + 1 <= j) hi = m.m[hh][at + 1][q][lane];
-              fm[q] = bf16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-            }
+            for (int q = 0; q < Q; ++q) fm[q] = *(const bf16x8*)&m.m[hh][S::m_at(2 * k, j, q, lane)];
             acc[j] = mma<R, Q, Q>(fx[k], fm, acc[j]);
+          }
+          if (j % 2 == 0) {
+            bf16x4 fm[Q];
+#pragma unroll
+            for (int q = 0; q < Q; ++q) fm[q] = m.m[hh][S::m_at(j, j, q, lane)];
+            acc[j] = mma_half<R, Q, Q>(fx[j / 2], fm, acc[j]);
           }
           if (j % 2) __builtin_amdgcn_sched_barrier(0);
         }
