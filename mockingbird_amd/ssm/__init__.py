@@ -81,15 +81,16 @@ def _numbers(fn, name, t, dtype, n):
     """A device list of n row numbers / flags; None stays None."""
     if t is None:
         return None
-    if t.dtype is not dtype or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
-        _refuse(f"{fn}: {name} must be a contiguous {dtype} tensor of {n}, got {t.dtype} {list(t.shape)}")
-    return t.data_ptr()
+    if t.dtype is dtype and t.shape == (n,) and t.is_contiguous():
+        return t.data_ptr()
+    _refuse(f"{fn}: {name} must be a contiguous {dtype} tensor of {n}, got {t.dtype} {list(t.shape)}")
 
 
 def _rows(fn, name, t, lead, tail, dtype):
     """(batch stride, row stride) of a tensor of `lead` rows of `tail`, dense within a row."""
-    st = t.stride()
-    if t.dtype is dtype and t.shape == lead + tail and st[-1] == 1 and (len(tail) == 1 or (len(tail) == 2 and st[-2] == tail[1])):
+    st, k = t.stride(), len(tail)
+    if t.dtype is dtype and t.shape == lead + tail and st[-1] == 1 and (k == 1 or (st[-2] == tail[-1] and (
+            k == 2 or st[-3] == tail[-1] * tail[-2]))):
         return (st[0], st[1]) if len(lead) == 2 else (0, st[0])
     if t.dtype is not dtype:
         _refuse(f"{fn}: {name} is {t.dtype}, expected {dtype}")
@@ -102,6 +103,11 @@ def _rows(fn, name, t, lead, tail, dtype):
         dense *= tail[-1 - i]
     n = len(lead)
     return (st[0] if n == 2 else 0), st[n - 1]
+
+
+def _fresh(x, lead, tail, bstride, rstride):
+    """A new contiguous output of x's type with its (batch stride, row stride)."""
+    return (torch.empty_like(x) if x.is_contiguous() else x.new_empty(lead + tail)), bstride, rstride
 
 
 def _extent(t):
@@ -147,12 +153,15 @@ def _other_columns(out, t, lead, row, off):
     return off >= row * e and off + width <= step
 
 
-_raw_stream = torch._C._cuda_getCurrentRawStream  # torch.cuda.current_stream(index).cuda_stream, without the object around it
+# torch.cuda.current_stream(index).cuda_stream and torch.cuda.current_device() without the objects and the start-up check around them (there
+# are tensors on the device).  A call of one token is a few microseconds of kernel: what the host spends per call is most of its time.
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_device = torch._C._cuda_getDevice
 
 
 def _launch(fn, index, call, *args):
     """The call on the current stream of the tensors' device."""
-    if index == torch.cuda.current_device():
+    if index == _device():
         rc = call(*args, _raw_stream(index))
     else:
         with torch.cuda.device(index):
@@ -183,19 +192,17 @@ def _pool(fn, state, dtype, inner, batch, slots, has_state):
         if slots is not None or has_state is not None:
             _refuse(f"{fn}: slots and has_state belong to a state pool")
         return None, 0, 0, None, None
-    if state.dim() != 1 + len(inner):
-        _refuse(f"{fn}: state must have shape [slots, {', '.join(map(str, inner))}], got {list(state.shape)}")
-    n = state.shape[0]
-    _, stride = _rows(fn, "state", state, (n,), inner, dtype)
-    size = 1
-    for v in inner:
-        size *= v
-    if n > 1 and stride < size:
+    shape = state.shape
+    if len(shape) != 1 + len(inner):
+        _refuse(f"{fn}: state must have shape [slots, {', '.join(map(str, inner))}], got {list(shape)}")
+    n = shape[0]
+    stride = _rows(fn, "state", state, (n,), inner, dtype)[1]
+    if n > 1 and stride < (inner[0] * inner[1] if len(inner) == 2 else inner[0] * inner[1] * inner[2]):
         _refuse(f"{fn}: state's slots overlap each other (strides {state.stride()})")
     if slots is None and batch > n:
         _refuse(f"{fn}: {batch} requests without slots, but a pool of {n}")
-    return (state.data_ptr(), stride, n, _numbers(fn, "slots", slots, torch.int32, batch),
-            _numbers(fn, "has_state", has_state, torch.bool, batch))
+    return (state.data_ptr(), stride, n, None if slots is None else _numbers(fn, "slots", slots, torch.int32, batch),
+            None if has_state is None else _numbers(fn, "has_state", has_state, torch.bool, batch))
 
 
 def _conv_weight(fn, weight, channels):
@@ -230,10 +237,10 @@ def causal_conv1d(x, weight, bias=None, activation=None, *, cu_seqlens=None, len
     w, k = _conv_weight(fn, weight, c)
     st, st_stride, n_slots, sl, has = _pool(fn, state, x.dtype, (k - 1, c), batch, slots, has_state)
     if out is None:
-        out = x.new_empty(lead + (c,))
+        out, yb, yr = _fresh(x, lead, (c,), t * c, c)
     else:
         _apart(fn, out, lead, c, ("x", x), ("state", state))
-    yb, yr = _rows(fn, "out", out, lead, (c,), x.dtype)
+        yb, yr = _rows(fn, "out", out, lead, (c,), x.dtype)
     a = _lib.CausalConv1dArgs(x.data_ptr(), out.data_ptr(), w, _param(fn, "bias", bias, c), st, sl, has, cu, valid, xb, xr, yb, yr,
                               st_stride, _DTYPES[x.dtype], batch, t, c, k, _activation(fn, activation), n_slots)
     _launch(fn, index, _lib.lib().mb_causal_conv1d, C.byref(a))
@@ -253,10 +260,10 @@ def causal_conv1d_step(x, state, weight, bias=None, activation=None, *, slots=No
     w, k = _conv_weight(fn, weight, c)
     st, st_stride, n_slots, sl, _ = _pool(fn, state, x.dtype, (k - 1, c), b, slots, None)
     if out is None:
-        out = x.new_empty((b, c))
+        out, _, yr = _fresh(x, (b,), (c,), 0, c)
     else:
         _apart(fn, out, (b,), c, ("x", x), ("state", state))
-    _, yr = _rows(fn, "out", out, (b,), (c,), x.dtype)
+        _, yr = _rows(fn, "out", out, (b,), (c,), x.dtype)
     a = _lib.CausalConv1dArgs(x.data_ptr(), out.data_ptr(), w, _param(fn, "bias", bias, c), st, sl, None, None, None, 0, xr, 0, yr,
                               st_stride, _DTYPES[x.dtype], b, 1, c, k, _activation(fn, activation), n_slots)
     _launch(fn, index, _lib.lib().mb_causal_conv1d_step, C.byref(a))
@@ -295,10 +302,10 @@ def _scan_args(fn, step, x, dt, A, B, C_, D, dt_bias, dt_softplus, dt_limit, cu_
     cb, cr = _rows(fn, "C", C_, lead, (g, n), x.dtype)
     st, st_stride, n_slots, sl, has = _pool(fn, state, torch.float32, (h, p, n), batch, slots, has_state)
     if out is None:
-        out = x.new_empty(lead + (h, p))
+        out, yb, yr = _fresh(x, lead, (h, p), t * h * p, h * p)
     else:
         _apart(fn, out, lead, h * p, ("x", x), ("dt", dt), ("B", B), ("C", C_), ("state", state))
-    yb, yr = _rows(fn, "out", out, lead, (h, p), x.dtype)
+        yb, yr = _rows(fn, "out", out, lead, (h, p), x.dtype)
     a = _lib.SelectiveScanArgs(x.data_ptr(), out.data_ptr(), dt.data_ptr(), B.data_ptr(), C_.data_ptr(), _param(fn, "A", A, h),
                                _param(fn, "D", D, h), _param(fn, "dt_bias", dt_bias, h), st, sl, has, cu, valid, xb, xr, yb, yr, db, dr,
                                bb, br, cb, cr, st_stride, _DTYPES[x.dtype], _DTYPES[dt.dtype], batch, t, h, p, g, n, n_slots,
@@ -336,6 +343,8 @@ def _row_stride(fn, name, t, shape, dtype):
         _refuse(f"{fn}: {name} is {t.dtype}, expected {dtype}")
     if t.shape != shape:
         _refuse(f"{fn}: {name} has shape {list(t.shape)}, expected {list(shape)}")
+    if t.is_contiguous():
+        return shape[-1]
     st = t.stride()
     if len(st) == 2 and st[1] == 1 and shape[0] > 1:
         return st[0]
@@ -395,17 +404,17 @@ def block_norm(x, weight=None, bias=None, *, norm="rms", eps=1e-5, groups=1, gat
         _refuse(f"{fn}: {c} channels in {groups!r} groups (1..1024 equal ones, of the first norm)")
     if norm is None and next_norm is None and residual is None and gate is None:
         _refuse(f"{fn}: nothing to compute")
-    xs = _row_stride(fn, "x", x, shape, x.dtype)
-    reads = [("x", x, xs)]
+    dtype = sum_dtype = x.dtype
+    xs = _row_stride(fn, "x", x, shape, dtype)
     gs = rs = 0
     if gate is not None:
-        gs = _row_stride(fn, "gate", gate, shape, x.dtype)
-        reads.append(("gate", gate, gs))
-    sum_dtype = x.dtype
+        gs = _row_stride(fn, "gate", gate, shape, dtype)
     if residual is not None:
-        sum_dtype = torch.float32 if residual.dtype is torch.float32 else x.dtype
+        if residual.dtype is _F32:
+            sum_dtype = _F32
         rs = _row_stride(fn, "residual", residual, shape, sum_dtype)
-        reads.append(("residual", residual, rs))
+    reads = [(name, t, st) for name, t, st in (("x", x, xs), ("gate", gate, gs), ("residual", residual, rs)) if t is not None] \
+        if out is not None or residual_out is not None else ()
     if next_norm is None:
         if out is not None and residual_out is not None:
             _refuse(f"{fn}: without next_norm there is one result: out or residual_out")
@@ -414,7 +423,8 @@ def block_norm(x, weight=None, bias=None, *, norm="rms", eps=1e-5, groups=1, gat
         total, y = residual_out, out
     rows = x.numel() // c if c else 0
     if total is None:
-        total, ss = x.new_empty(tuple(shape), dtype=sum_dtype), c
+        like = x if residual is None else residual  # of the sum's type
+        total, ss = (torch.empty_like(like) if like.is_contiguous() else like.new_empty(shape)), c
     else:
         ss = _row_stride(fn, "residual_out" if next_norm or residual_out is not None else "out", total, shape, sum_dtype)
         if rows > 1 and ss < c:
@@ -423,17 +433,17 @@ def block_norm(x, weight=None, bias=None, *, norm="rms", eps=1e-5, groups=1, gat
     ys = 0
     if next_norm is not None:
         if y is None:
-            y, ys = x.new_empty(tuple(shape)), c
+            y, ys = (torch.empty_like(x) if x.is_contiguous() else x.new_empty(shape)), c
         else:
-            ys = _row_stride(fn, "out", y, shape, x.dtype)
+            ys = _row_stride(fn, "out", y, shape, dtype)
             if rows > 1 and ys < c:
                 _refuse(f"{fn}: out's rows overlap each other")
-            _same_or_apart(fn, "out", y, ys, reads + [("*the sum", total, ss)])
+            _same_or_apart(fn, "out", y, ys, [*reads, ("*the sum", total, ss)])
     a = _lib.BlockNormArgs(x.data_ptr(), None if gate is None else gate.data_ptr(), None if residual is None else residual.data_ptr(),
                            total.data_ptr(), None if y is None else y.data_ptr(), _param(fn, "weight", weight, c),
                            _param(fn, "bias", bias, c), _param(fn, "scale", scale, c) if vec else None,
                            _param(fn, "next_weight", next_weight, c), _param(fn, "next_bias", next_bias, c), rows, xs, gs, rs, ss, ys,
-                           _DTYPES[x.dtype], _DTYPES[sum_dtype], c, groups, _NORMS[norm], _NORMS[next_norm], _GATES[gate_act],
+                           _DTYPES[dtype], _DTYPES[sum_dtype], c, groups, _NORMS[norm], _NORMS[next_norm], _GATES[gate_act],
                            1 if gate_first else 0, eps, next_eps, 1.0 if scale is None or vec else float(scale))
     _launch(fn, index, _lib.lib().mb_block_norm, C.byref(a))
     return total if y is None else (total, y)
