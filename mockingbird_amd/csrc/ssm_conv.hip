@@ -151,6 +151,8 @@ template <typename T, int K> int launch_conv(const mb_causal_conv1d_args& a, boo
     const int nv = cdiv(a.channels, CONV_V);
     int cx = 16;
     while (cx < 256 && cx < nv) cx *= 2;
+    // narrower where that leaves fewer threads without a channel (4352 channels, 16 k rows: 64 side by side 57 us, 256 59 us; 32 no better)
+    while (cx > 64 && cdiv(nv, cx / 2) * (cx / 2) < cdiv(nv, cx) * cx) cx /= 2;
     // longer runs read fewer rows twice; shorter ones give every CU several workgroups
     const Rows rows = {a.d_cu_seqlens, a.d_valid, a.batch, a.t};
     int R = 32;
