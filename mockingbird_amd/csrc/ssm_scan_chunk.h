@@ -11,12 +11,14 @@
 // order: x^T by transposing reads of rows 4 g + i and 16 + 4 g + i; for C h the state's rows are numbered so that the order is C's own
 // (tile 2 q holds columns 32 q + 8 g + i, tile 2 q + 1 those 4 further on).
 //
-// What bounds it is the vector pipe, which splits h, M and c x into planes (about 560 instructions per wave and chunk beside 91 matrix
-// instructions), and the order of a chunk: step sizes, G, M, M x.  Hence: M is formed once per head and goes through LDS; two
+// What bounds it: per wave and chunk 97 matrix instructions and about 560 vector ones, most of which split h, M and c x into planes, take 28 %
+// and 40 % of the time of their pipes and overlap by half at best; the rest is the order of a chunk -- step sizes, G, M, M x, three meetings of
+// the waves (39 % of their time is waiting; 60 vector instructions fewer gave 1 %).  Hence: M is formed once per head and goes through LDS; two
 // workgroups of 8 waves fit a CU (78 KB of LDS, 128 registers, nothing spilled -- a reload waits for the loads in flight in front of it),
 // so that one's products run while the other waits; the terms of the step sizes are a chunk ahead; the conversion of the next operand
 // stands between the products of this one.  Four waves of 32 columns read LDS half as often and are no faster (8192 rows, 64 heads of
-// 64 x 128: 149 and 146 us), one workgroup of four heads neither.
+// 64 x 128: 149 and 146 us), one workgroup of four heads neither, nor the second pass adding up the tiles in front of its own instead of a
+// join (156 and 137 us).
 // Measured, 8192 rows x 64 heads of 64 columns, 128 states, bf16: 80 us this pass, 41 us the states' pass, 13 us the join between them, of
 // 28 us that its bytes take at a large copy's rate.  Planes less would save 9 us (h and M in one) and 10 us (c x in two) of it.
 //
