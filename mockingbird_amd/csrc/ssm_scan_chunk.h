@@ -116,20 +116,6 @@ __device__ __forceinline__ f32x4 mma(const bf16x8 (&a)[QA], const bf16x8 (&b)[QB
   return acc;
 }
 
-// the same with the first 16 of a's 32 rows
-template <int QA, int QB, int K>
-__device__ __forceinline__ f32x4 mma_half(const bf16x8 (&a)[QA], const bf16x4 (&b)[QB], f32x4 acc) {
-#pragma unroll
-  for (int i = QA - 1; i >= 0; --i)
-#pragma unroll
-    for (int j = QB - 1; j >= 0; --j)
-      if (i + j < K) {
-        const bf16x4 lo = {a[i][0], a[i][1], a[i][2], a[i][3]};
-        acc = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(s16x4, lo), __builtin_bit_cast(s16x4, b[j]), acc, 0, 0, 0);
-      }
-  return acc;
-}
-
 template <typename T, int NP, bool STATES> struct ScanShape {
   static constexpr int R = sizeof(T) == 4 ? 3 : std::is_same<T, f16>::value ? 2 : 1;  // raw planes
   static constexpr int Q = R == 3 ? 3 : 2;                                             // planes of M and h
@@ -618,10 +604,15 @@ __global__ __launch_bounds__((ScanShape<T, NP, STATES>::THREADS), (ScanShape<T, 
             acc[j] = mma<R, Q, Q>(fx[k], fm, acc[j]);
           }
           if (j % 2 == 0) {
-            bf16x4 fm[Q];
+            // 16 rows and 16 zeros, not the 16-row instruction: behind one of 32 rows on the same accumulators, with nothing between, it gave
+            // wrong sums now and then
+            bf16x8 fm[Q];
 #pragma unroll
-            for (int q = 0; q < Q; ++q) fm[q] = m.m[hh][S::m_at(j, j, q, lane)];
-            acc[j] = mma_half<R, Q, Q>(fx[j / 2], fm, acc[j]);
+            for (int q = 0; q < Q; ++q) {
+              const bf16x4 lo = m.m[hh][S::m_at(j, j, q, lane)];
+              fm[q] = bf16x8{lo[0], lo[1], lo[2], lo[3], (__bf16)0.f, (__bf16)0.f, (__bf16)0.f, (__bf16)0.f};
+            }
+            acc[j] = mma<R, Q, Q>(fx[j / 2], fm, acc[j]);
           }
           if (j % 2) __builtin_amdgcn_sched_barrier(0);
         }
