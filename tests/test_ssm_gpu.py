@@ -768,3 +768,29 @@ def test_refusals_of_steps_and_devices():
         ssm.block_norm(x, p)
     with torch.no_grad():
         assert ssm.block_norm(x, p).shape == x.shape
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_selective_scan_repeats_to_the_bit_in_any_order(dtype):
+    """Calls of many shapes behind each other in changing orders, on fresh copies of their inputs: what a call gives does not depend on what
+    the chip did before it."""
+    import random
+    from mockingbird_amd import ssm
+    rng, r = random.Random(11), gen(11)
+    calls = []
+    for _ in range(200):
+        h, p, n = rng.randint(1, 24), rng.choice([32, 40, 64, 96, 128]), rng.choice([24, 64, 64, 128])
+        lens = [rng.randint(1, 130) for _ in range(rng.randint(1, 5))]
+        cu = torch.tensor([sum(lens[:i]) for i in range(len(lens) + 1)], dtype=torch.int32).cuda()
+        x, dt, a, bm, cm, skip, bias = (t.cuda() for t in scan_inputs(r, (sum(lens),), h, p, n, 1, dtype))
+        calls.append(((x, dt, a, bm, cm, skip), dict(dt_bias=bias, dt_softplus=True, cu_seqlens=cu)))
+    want = [None] * len(calls)
+    for turn in range(8):
+        order = list(range(len(calls)))
+        rng.shuffle(order)
+        for i in order:
+            args, kw = calls[i]
+            got = ssm.selective_scan(*[t.clone() for t in args], **kw)
+            if want[i] is None:
+                want[i] = got
+            assert torch.equal(got, want[i]), (turn, i, list(args[0].shape), list(args[3].shape))
