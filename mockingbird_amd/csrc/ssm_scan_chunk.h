@@ -11,7 +11,7 @@
 // order: x^T by transposing reads of rows 4 g + i and 16 + 4 g + i; for C h the state's rows are numbered so that the order is C's own
 // (tile 2 q holds columns 32 q + 8 g + i, tile 2 q + 1 those 4 further on).
 //
-// What bounds it: per wave and chunk 97 matrix instructions and about 560 vector ones, most of which split h, M and c x into planes, take 28 %
+// What bounds it: per wave and chunk 97 matrix instructions and about 570 vector ones, most of which split h, M and c x into planes, take 28 %
 // and 40 % of the time of their pipes and overlap by half at best; the rest is the order of a chunk -- step sizes, G, M, M x, three meetings of
 // the waves (39 % of their time is waiting; 60 vector instructions fewer gave 1 %).  Hence: M is formed once per head and goes through LDS; two
 // workgroups of 8 waves fit a CU (78 KB of LDS, 128 registers, nothing spilled -- a reload waits for the loads in flight in front of it),
