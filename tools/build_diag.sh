@@ -1,12 +1,19 @@
 #!/bin/bash
-# diagnostics build of libmbhip (intra-kernel marks): mockingbird_amd/libmbhip_diag.so
+# diagnostics build of libmbhip (intra-kernel marks): mockingbird_amd/libmbhip_diag.so.  Sources and flags are the library's own, plus the marks.
 set -e
 cd "$(dirname "$0")/../mockingbird_amd/csrc"
+HIPCC=${HIPCC:-/opt/rocm/bin/hipcc}
+FLAGS=$(python3 -c 'import sys; sys.path.insert(0, ".."); import build; print(*build.FLAGS)')
+SOURCES=$(python3 -c 'import sys; sys.path.insert(0, ".."); import build; print(*build.SOURCES)')
+tmp=$(mktemp -d)
+trap 'rm -rf "$tmp"' EXIT
 objs=""
-for f in common conv1d gan rnn wavernn tacotron maximum_path; do
-  /opt/rocm/bin/hipcc -O3 -std=c++17 -fPIC --offload-arch=gfx950 -fno-gpu-rdc -DMB_TRACE_MARKS -c $f.hip -o /tmp/diag_$f.o &
-  objs="$objs /tmp/diag_$f.o"
+pids=""
+for f in $SOURCES; do
+  $HIPCC $FLAGS -DMB_TRACE_MARKS -c $f -o $tmp/${f%.hip}.o &
+  pids="$pids $!"
+  objs="$objs $tmp/${f%.hip}.o"
 done
-wait
-/opt/rocm/bin/hipcc -shared -fPIC --offload-arch=gfx950 -o ../libmbhip_diag.so $objs
+for p in $pids; do wait $p; done
+$HIPCC -shared -fPIC --offload-arch=gfx950 -o ../libmbhip_diag.so $objs
 echo built ../libmbhip_diag.so

@@ -1,6 +1,6 @@
 // Is the instruction cache cold at every kernel launch?  A wave runs the SAME long straight-line
 // code twice inside one launch (pass 0, pass 1) and stamps shader clocks around each pass.
-// Build: hipcc -O3 --offload-arch=gfx950 icache.hip -o icache
+// Build: hipcc -O3 --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops icache.hip -o icache
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <vector>

@@ -3,7 +3,7 @@
 // recurrent GEMM, rnn_ts2_body.h) and stamps the shader clock (clock64, s_memtime) and the constant 100 MHz
 // wall clock (wall_clock64, s_memrealtime) around the loop.  cycles / wall time = sustained clock;
 // cycles / MFMA = issue cost (32 when nothing stalls).
-// Build: hipcc -O3 --offload-arch=gfx950 mfma_clock.hip -o mfma_clock ; run: ./mfma_clock
+// Build: hipcc -O3 --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops mfma_clock.hip -o mfma_clock ; run: ./mfma_clock
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <vector>

@@ -2,7 +2,7 @@
 // coherent) L2s.  NWG workgroups of 512 threads each read the SAME `bytes` region (an exchange vector every consumer needs),
 // once with plain 16-byte loads (L2 hits after the first toucher of each XCD: what a launch boundary gives) and once with
 // 8-byte relaxed agent-scope atomic loads (global_load_dwordx2 sc1: what a tagged-granule sweep issues).
-// build: hipcc -O3 --offload-arch=gfx950 tools/micro/sc1_gather.hip -o build_variants/sc1_gather ; run: build_variants/sc1_gather
+// build: hipcc -O3 --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops tools/micro/sc1_gather.hip -o build_variants/sc1_gather ; run: build_variants/sc1_gather
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <vector>
