@@ -148,6 +148,8 @@ def _other_columns(out, t, lead, row, off):
     if not strides or t.element_size() != e or tuple(t.shape[:k]) != lead or any(
             n > 1 and p != q for n, p, q in zip(lead, t.stride(), out.stride())):
         return False
+    if any(st % strides[0] for st in strides):  # a batch starts inside a row of the others: columns do not tell them apart
+        return False
     step, width = strides[0] * e, t[(0,) * k].numel() * e
     off %= step
     return off >= row * e and off + width <= step
