@@ -778,6 +778,8 @@ int mb_wave_finish_batch(const float* d_wav, const long long* d_pieces, int n_pi
  *    State pools: [n_slots] states, item b owns slot d_slots[b] (NULL: slot b).  An item whose slot is outside 0..n_slots-1, or is named
  *    by an earlier item of the call too, is left out: neither its rows nor a state are written.  d_has_state[b] == 0: the item starts from
  *    zeros whatever its slot holds (NULL: every item continues).  A state is updated in place, also that of an item without rows.
+ *    What a call writes (outputs, states, workspace) shares no memory with anything else it takes, or the call is refused; other columns of the
+ *    same rows are fine, and mb_block_norm's outputs may be its inputs.
  *    All calls only enqueue kernels on `stream` and may be captured into a graph.
  * ---------------------------------------------------------------------- */
 #define MB_BF16 3
@@ -785,7 +787,7 @@ int mb_wave_finish_batch(const float* d_wav, const long long* d_pieces, int n_pi
 /* y[t][c] = act(bias[c] + sum_j w[c][j] * x[t - ksize + 1 + j][c]); rows before an item's first one are its state's. */
 typedef struct mb_causal_conv1d_args {
   const void* d_x;           /* rows of [channels]                                             */
-  void* d_y;                 /* rows of [channels], must not overlap x                         */
+  void* d_y;                 /* rows of [channels]                                             */
   const float* d_w;          /* fp32 [channels][ksize]                                         */
   const float* d_bias;       /* fp32 [channels] or NULL                                        */
   void* d_state;             /* [n_slots][ksize - 1][channels] of `dtype`: the last inputs, oldest first; NULL: none */
@@ -800,7 +802,7 @@ int mb_causal_conv1d_step(const mb_causal_conv1d_args* a, mb_stream_t stream);
 /* Per head: d = dt + dt_bias, through softplus if asked for, clamped to [dt_min, dt_max]; h = exp(d * A) * h + (d * x) B^T; y = h C + D * x.
  * x, y: rows of [heads][head_dim]; dt: rows of [heads]; B, C: rows of [groups][d_state], head i reads group i / (heads / groups). */
 typedef struct mb_selective_scan_args {
-  const void* d_x; void* d_y; /* must not overlap any input                                    */
+  const void* d_x; void* d_y;
   const void* d_dt; const void* d_b; const void* d_c;
   const float* d_a; const float* d_d; const float* d_dt_bias;  /* fp32 [heads]; d_d, d_dt_bias may be NULL */
   float* d_state;             /* fp32 [n_slots][heads][head_dim][d_state] or NULL              */
@@ -819,7 +821,7 @@ int mb_selective_scan_step(const mb_selective_scan_args* a, mb_stream_t stream);
  * norm / next_norm: 0 none, 1 RMS, 2 layer norm (weight and bias NULL: ones and zeros); `groups`: the first norm over each of that many
  * equal parts of the row.  d_gate, d_residual NULL: without; scale = res_scale * d_scale[c] (NULL: 1).  d_sum receives s (NULL: not
  * stored), d_y the result of next_norm (only with next_norm).  x, gate and y are `dtype`; residual and sum `res_dtype` (dtype or MB_F32).
- * An output may be exactly one of the inputs, otherwise nothing overlaps. */
+ * An output may be exactly one of x, gate and residual. */
 typedef struct mb_block_norm_args {
   const void* d_x; const void* d_gate; const void* d_residual; void* d_sum; void* d_y;
   const float* d_weight; const float* d_bias; const float* d_scale; const float* d_next_weight; const float* d_next_bias;  /* fp32 [channels] */

@@ -154,7 +154,67 @@ __device__ __forceinline__ int slot_of(const int* slots, int b, int n_slots) {
   return __any(twice) ? -1 : s;
 }
 
+// A tensor of a call, for the check of what shares memory: a run of `bytes`, repeated along up to three axes (innermost first).
+struct Span {
+  const char* name;
+  const void* p;
+  long long bytes, n[3], stride[3];
+};
+static inline Span span_of(const char* name, const void* p, size_t elem, long long run, long long n0 = 1, long long s0 = 0, long long n1 = 1, long long s1 = 0) {
+  return {name, p, run * (long long)elem, {n0, n1, 1}, {s0 * (long long)elem, s1 * (long long)elem, 0}};
+}
+// Its address range; empty without a tensor.
+static inline void range_of(const Span& s, __int128& lo, __int128& hi) {
+  lo = hi = (__int128)(size_t)s.p;
+  if (!s.p || s.bytes <= 0) return;
+  __int128 down = 0, up = s.bytes;
+  for (int i = 0; i < 3; ++i) {
+    if (s.n[i] <= 0) return;
+    (s.stride[i] < 0 ? down : up) += (__int128)(s.n[i] - 1) * s.stride[i];
+  }
+  lo += down, hi += up;
+}
+// Two tensors whose ranges overlap share nothing if both repeat a run at multiples of one step (rows of a wider buffer) and the runs lie in
+// different columns of it.
+static inline bool other_columns(const Span& a, const Span& b) {
+  const Span* const s[2] = {&a, &b};
+  __int128 run[2], front[2][3], step = 0;
+  int axes[2];
+  for (int k = 0; k < 2; ++k) {
+    run[k] = s[k]->bytes, axes[k] = 0;
+    for (int i = 0; i < 3; ++i) {
+      const __int128 n = s[k]->n[i], st = s[k]->stride[i] < 0 ? -(__int128)s[k]->stride[i] : s[k]->stride[i];
+      if (n == 1) continue;
+      if (!axes[k] && s[k]->stride[i] == run[k]) {
+        run[k] *= n;
+      } else {
+        front[k][axes[k]++] = st;
+        if (st && (!step || st < step)) step = st;
+      }
+    }
+  }
+  if (!step) return false;
+  for (int k = 0; k < 2; ++k)
+    for (int i = 0; i < axes[k]; ++i)
+      if (front[k][i] % step) return false;
+  const __int128 off = (((__int128)(size_t)b.p - (__int128)(size_t)a.p) % step + step) % step;
+  return off >= run[0] && off + run[1] <= step;
+}
+// What a call writes (the first `written` spans) overlaps none of its other tensors; from `same` on a span may be exactly a written one.
+static inline int check_apart(const char* fn, const Span* s, int written, int all, int same = 16) {
+  __int128 lo[16], hi[16];
+  for (int i = 0; i < all; ++i) range_of(s[i], lo[i], hi[i]);
+  for (int i = 0; i < written; ++i)
+    for (int j = i + 1; j < all; ++j) {
+      if (lo[i] >= hi[j] || lo[j] >= hi[i]) continue;
+      const bool equal = j >= same && s[i].p == s[j].p && s[i].bytes == s[j].bytes && (s[i].n[0] == 1 || s[i].stride[0] == s[j].stride[0]);
+      MB_REQUIRE(equal || other_columns(s[i], s[j]), "%s: %s overlaps %s", fn, s[i].name, s[j].name);
+    }
+  return MB_OK;
+}
+
 __host__ __device__ static inline bool aligned(const void* p, size_t n) { return ((size_t)p & (n - 1)) == 0; }
+static inline size_t size_of(int dtype) { return dtype == MB_F32 ? 4 : 2; }
 
 }  // namespace ssm
 }  // namespace mb

@@ -142,10 +142,27 @@ __global__ __launch_bounds__(64) void causal_conv1d_step_kernel(const mb_causal_
   store_some<T, V>(st + (long long)(K - 2) * a.channels, cur, n);
 }
 
+static int conv_apart(const char* name, const mb_causal_conv1d_args& a, bool step) {
+  const size_t e = size_of(a.dtype);
+  const bool padded = !step && !a.d_cu_seqlens;
+  const long long rows = step ? a.batch : a.t, items = padded ? a.batch : 1;
+  const Span s[] = {span_of("out", a.d_y, e, a.channels, rows, a.y_rstride, items, a.y_bstride),
+                    span_of("state", a.d_state, e, (long long)(a.ksize - 1) * a.channels, a.n_slots, a.state_stride),
+                    span_of("x", a.d_x, e, a.channels, rows, a.x_rstride, items, a.x_bstride),
+                    span_of("weight", a.d_w, 4, (long long)a.channels * a.ksize),
+                    span_of("bias", a.d_bias, 4, a.channels),
+                    span_of("slots", a.d_slots, 4, a.batch),
+                    span_of("has_state", step ? nullptr : a.d_has_state, 1, a.batch),
+                    span_of("cu_seqlens", step ? nullptr : a.d_cu_seqlens, 4, a.batch + 1ll),
+                    span_of("lengths", step ? nullptr : a.d_valid, 4, a.batch)};
+  return check_apart(name, s, 2, sizeof(s) / sizeof(*s));
+}
+
 template <typename T, int K> int launch_conv(const mb_causal_conv1d_args& a, bool step, hipStream_t s) {
   if (step) {
     const long long grid = (long long)a.batch * cdiv(a.channels, 64 * CONV_V);
     MB_REQUIRE(grid < (1ll << 31), "causal_conv1d_step: %d items of %d channels are too many for one launch", a.batch, a.channels);
+    if (const int rc = conv_apart("causal_conv1d_step", a, true)) return rc;
     hipLaunchKernelGGL((causal_conv1d_step_kernel<T, K>), dim3((unsigned)grid), dim3(64), 0, s, a);
   } else {
     const int nv = cdiv(a.channels, CONV_V);
@@ -159,6 +176,7 @@ template <typename T, int K> int launch_conv(const mb_causal_conv1d_args& a, boo
     while (R > 8 && tiles_of(rows, R * (256 / cx)) * cdiv(nv, cx) < 2048) R /= 2;
     const long long grid = tiles_of(rows, R * (256 / cx)) * cdiv(nv, cx);
     MB_REQUIRE(grid < (1ll << 31), "causal_conv1d: %d rows of %d channels are too many for one launch", a.t, a.channels);
+    if (const int rc = conv_apart("causal_conv1d", a, false)) return rc;
     hipLaunchKernelGGL((causal_conv1d_kernel<T, K>), dim3((unsigned)grid), dim3(256), 0, s, a, cx, R);
   }
   MB_HIP(hipGetLastError());

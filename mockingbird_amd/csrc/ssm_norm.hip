@@ -276,6 +276,22 @@ template <typename T, typename TR> int launch_norm(const mb_block_norm_args& a, 
   return MB_OK;
 }
 
+// An output is exactly one of x, gate and residual (a thread reads an element before it writes it), or overlaps nothing.
+static int norm_apart(const mb_block_norm_args& a) {
+  const size_t e = size_of(a.dtype), r = size_of(a.res_dtype);
+  const Span s[] = {span_of("the sum", a.d_sum, r, a.channels, a.rows, a.sum_rstride),
+                    span_of("out", a.d_y, e, a.channels, a.rows, a.y_rstride),
+                    span_of("weight", a.d_weight, 4, a.channels),
+                    span_of("bias", a.d_bias, 4, a.channels),
+                    span_of("scale", a.d_scale, 4, a.channels),
+                    span_of("next_weight", a.d_next_weight, 4, a.channels),
+                    span_of("next_bias", a.d_next_bias, 4, a.channels),
+                    span_of("x", a.d_x, e, a.channels, a.rows, a.x_rstride),
+                    span_of("gate", a.d_gate, e, a.channels, a.rows, a.gate_rstride),
+                    span_of("residual", a.d_residual, r, a.channels, a.rows, a.residual_rstride)};
+  return check_apart("block_norm", s, 2, 10, 7);
+}
+
 static int check_norm(const mb_block_norm_args* a) {
   MB_REQUIRE(a, "block_norm: null arguments");
   MB_REQUIRE(a->dtype == MB_F32 || a->dtype == MB_F16 || a->dtype == MB_BF16, "block_norm: dtype %d is none of MB_F32, MB_F16, MB_BF16", a->dtype);
@@ -301,6 +317,7 @@ extern "C" int mb_block_norm(const mb_block_norm_args* a, mb_stream_t stream) {
   using namespace mb::ssm;
   const int go = check_norm(a);
   if (go <= 0) return go;
+  if (const int rc = norm_apart(*a)) return rc;
   hipStream_t s = (hipStream_t)stream;
   if (a->dtype == MB_F32) return launch_norm<float, float>(*a, s);
   if (a->dtype == MB_F16) return a->res_dtype == MB_F32 ? launch_norm<f16, float>(*a, s) : launch_norm<f16, f16>(*a, s);

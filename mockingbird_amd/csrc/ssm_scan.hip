@@ -187,6 +187,27 @@ static int check_scan(const char* name, const mb_selective_scan_args* a, bool st
   return 1;
 }
 
+static int scan_apart(const char* name, const mb_selective_scan_args& a, bool step, const void* ws, size_t ws_bytes) {
+  const size_t e = size_of(a.dtype);
+  const bool padded = !step && !a.d_cu_seqlens;
+  const long long rows = step ? a.batch : a.t, items = padded ? a.batch : 1, wide = (long long)a.heads * a.head_dim, narrow = (long long)a.groups * a.d_state_dim;
+  const Span s[] = {span_of("out", a.d_y, e, wide, rows, a.y_rstride, items, a.y_bstride),
+                    span_of("state", a.d_state, 4, wide * a.d_state_dim, a.n_slots, a.state_stride),
+                    span_of("the workspace", ws, 1, (long long)ws_bytes),
+                    span_of("x", a.d_x, e, wide, rows, a.x_rstride, items, a.x_bstride),
+                    span_of("dt", a.d_dt, size_of(a.dt_dtype), a.heads, rows, a.dt_rstride, items, a.dt_bstride),
+                    span_of("B", a.d_b, e, narrow, rows, a.b_rstride, items, a.b_bstride),
+                    span_of("C", a.d_c, e, narrow, rows, a.c_rstride, items, a.c_bstride),
+                    span_of("A", a.d_a, 4, a.heads),
+                    span_of("D", a.d_d, 4, a.heads),
+                    span_of("dt_bias", a.d_dt_bias, 4, a.heads),
+                    span_of("slots", a.d_slots, 4, a.batch),
+                    span_of("has_state", step ? nullptr : a.d_has_state, 1, a.batch),
+                    span_of("cu_seqlens", step ? nullptr : a.d_cu_seqlens, 4, a.batch + 1ll),
+                    span_of("lengths", step ? nullptr : a.d_valid, 4, a.batch)};
+  return check_apart(name, s, 3, sizeof(s) / sizeof(*s));
+}
+
 static int run_scan(const mb_selective_scan_args* a, void* ws, size_t ws_bytes, hipStream_t s) {
   const int go = check_scan("selective_scan", a, false);
   if (go <= 0) return go;
@@ -197,6 +218,7 @@ static int run_scan(const mb_selective_scan_args* a, void* ws, size_t ws_bytes, 
     return MB_ENOMEM;
   }
   MB_REQUIRE(aligned(ws, 16), "selective_scan: the workspace must be 16-byte aligned");
+  if (const int rc = scan_apart("selective_scan", *a, false, ws, need)) return rc;
   auto* chunks = a->dtype == MB_F32 ? scan_chunks_f32 : a->dtype == MB_F16 ? scan_chunks_f16 : scan_chunks_bf16;
   if (sp.seg) {
     const int rc = chunks(*a, sp, true, s);
@@ -212,6 +234,7 @@ static int run_scan(const mb_selective_scan_args* a, void* ws, size_t ws_bytes, 
 static int run_step(const mb_selective_scan_args* a, hipStream_t s) {
   const int go = check_scan("selective_scan_step", a, true);
   if (go <= 0) return go;
+  if (const int rc = scan_apart("selective_scan_step", *a, true, nullptr, 0)) return rc;
   return a->dtype == MB_F32 ? step_by_lanes<float>(*a, s) : a->dtype == MB_F16 ? step_by_lanes<f16>(*a, s) : step_by_lanes<bf16>(*a, s);
 }
 

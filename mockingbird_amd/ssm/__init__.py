@@ -13,7 +13,8 @@ Activations are float32, float16 or bfloat16 CUDA(HIP) tensors, time-major and d
 projection).  Parameters and scan states are float32.  Packed requests are [rows, ...] with cu_seqlens (int32 [n + 1]), padded ones
 [batch, t, ...] with optional lengths (int32 [batch]); both stay on the device.  Rows that belong to no request are left as `out` held them
 (a fresh `out` is not initialised there).  state[slots[i]] is request i's state, updated in place; a request whose slot is outside the
-pool, or already named by an earlier request of the call, is left out.  has_state[i] == False starts request i from zeros.
+pool, or already named by an earlier request of the call, is left out.  has_state[i] == False starts request i from zeros.  What a call writes
+shares no memory with its other tensors (other columns of the same rows are fine).
 
 Inference only: a tensor that requires grad is refused while grad mode is on.  There is no CPU path."""
 import ctypes as C
@@ -124,8 +125,8 @@ def _extent(t):
 
 
 def _apart(fn, out, lead, row, *others):
-    """An output must not hold a row twice, nor overlap an input ((name, tensor) pairs) -- unless both are different columns of the same
-    rows."""
+    """An output must not hold a row twice, nor overlap another tensor of the call ((name, tensor) pairs) -- unless both are different columns
+    of the same rows.  (The library looks at everything else that a call writes and reads.)"""
     if not out.is_contiguous():
         need = row
         for st, n in sorted((st, n) for st, n in zip(out.stride()[:len(lead)], lead) if n > 1):
@@ -137,22 +138,32 @@ def _apart(fn, out, lead, row, *others):
         if t is None:
             continue
         a, b = _extent(t)
-        if lo < b and a < hi and not _other_columns(out, t, lead, row, a - lo):
+        if lo < b and a < hi and not _other_columns(out, t, a - lo):
             _refuse(f"{fn}: out overlaps {name}")
 
 
-def _other_columns(out, t, lead, row, off):
-    """t, `off` bytes behind out, holds other columns of the same rows."""
-    k, e = len(lead), out.element_size()
-    strides = sorted(st for st, n in zip(out.stride(), lead) if n > 1)
-    if not strides or t.element_size() != e or tuple(t.shape[:k]) != lead or any(
-            n > 1 and p != q for n, p, q in zip(lead, t.stride(), out.stride())):
+def _blocks(t):
+    """(bytes of the dense block that a tensor repeats, byte strides of the axes that repeat it)."""
+    e, width, front = t.element_size(), 1, []
+    for n, st in zip(reversed(t.shape), reversed(t.stride())):
+        if n == 1:
+            continue
+        if not front and st == width:
+            width *= n
+        else:
+            front.append(st * e)
+    return width * e, front
+
+
+def _other_columns(t, u, off):
+    """u, `off` bytes behind t, holds other columns of the same rows: both repeat a block at multiples of one row, and the blocks lie apart."""
+    (wt, ft), (wu, fu) = _blocks(t), _blocks(u)
+    steps = ft + fu
+    step = min((st for st in steps if st), default=0)
+    if not step or any(st % step for st in steps):  # (a batch that starts inside a row of the others: columns do not tell them apart)
         return False
-    if any(st % strides[0] for st in strides):  # a batch starts inside a row of the others: columns do not tell them apart
-        return False
-    step, width = strides[0] * e, t[(0,) * k].numel() * e
     off %= step
-    return off >= row * e and off + width <= step
+    return off >= wt and off + wu <= step
 
 
 # torch.cuda.current_stream(index).cuda_stream and torch.cuda.current_device() without the objects and the start-up check around them (there
