@@ -16,10 +16,11 @@ projection).  Parameters and scan states are float32.  Packed requests are [rows
 pool, or already named by an earlier request of the call, is left out.  has_state[i] == False starts request i from zeros.  What a call writes
 shares no memory with its other tensors (other columns of the same rows are fine).
 
-Inference only: a tensor that requires grad is refused while grad mode is on.  There is no CPU path."""
+Inference only: a tensor that requires grad is refused while grad mode is on, one with a forward-mode tangent always.  There is no CPU path."""
 import ctypes as C
 
 import torch
+from torch.autograd import forward_ad
 
 from .. import _lib
 
@@ -46,10 +47,19 @@ def _inputs(fn, x, **others):
                 good = good and t.get_device() == index
                 wanted = wanted or (grad and t.requires_grad)
         if good and not wanted:
+            if forward_ad._current_level >= 0:  # -1 outside of dual_level()
+                _refuse_tangents(fn, x=x, **others)
             return index
     except AttributeError:
         pass
     _refuse_inputs(fn, x, others)
+
+
+def _refuse_tangents(fn, **tensors):
+    """no_grad() does not keep forward-mode derivatives from being asked for; the results would carry none."""
+    for name, t in tensors.items():
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            _refuse(f"{fn} has no derivative: {name} is a dual tensor")
 
 
 def _refuse_inputs(fn, x, others):

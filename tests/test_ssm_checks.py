@@ -141,3 +141,37 @@ def test_slots_with_room_for_the_next_input_and_the_answer(cuda, lib):
         assert torch.equal(buf[:n, :K - 1], was[:n, 1:K]) and torch.equal(buf[:n, K - 1], was[:n, K - 1]) and torch.equal(buf[n:], was[n:])
         # four products with ones, each sum rounded
         assert (y.double() - was[:n, :K].double().sum(1)).abs().max() <= 4 * 2.0 ** -24 * was[:n, :K].abs().sum(1).max()
+
+
+def test_forward_mode_tangents_are_seen(lib):
+    from torch.autograd import forward_ad
+    from mockingbird_amd import _lib, ssm
+    x = torch.zeros(3)
+    with forward_ad.dual_level():
+        ssm._refuse_tangents("f", x=x, bias=None)
+        with pytest.raises(_lib.MbHipError, match="bias is a dual tensor"), torch.no_grad():
+            ssm._refuse_tangents("f", x=x, bias=forward_ad.make_dual(x, x))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("grad", [True, False])
+@pytest.mark.parametrize("i,arg", [(i, a) for i, (_, spec) in enumerate(arguments()) for a, (_, dtype) in spec.items() if dtype is F32 and a[:5] != "next_"])
+def test_forward_mode_derivatives_are_refused(cuda, lib, i, arg, grad):
+    from torch.autograd import forward_ad
+    from mockingbird_amd import _lib, ssm
+    name, spec = arguments()[i]
+    kw = {k: torch.zeros(shape, dtype=dtype, device="cuda") for k, (shape, dtype) in spec.items()}
+    if name == "block_norm":
+        kw.pop("next_weight"), kw.pop("next_bias")
+    if "cu_seqlens" in kw:  # every row belongs to a request: rows of a fresh output that belong to none hold anything
+        kw["cu_seqlens"].copy_(torch.tensor([0, 2, T]))
+    if "lengths" in kw:
+        kw["lengths"].fill_(T // 2)
+    if "slots" in kw:
+        kw["slots"].copy_(torch.arange(kw["slots"].numel()))
+    plain = getattr(ssm, name)(**kw)
+    with forward_ad.dual_level(), torch.set_grad_enabled(grad):
+        assert torch.equal(getattr(ssm, name)(**kw), plain)  # other tensors of the program have tangents, these have none
+        kw[arg] = forward_ad.make_dual(kw[arg], torch.ones_like(kw[arg]))
+        with pytest.raises(_lib.MbHipError, match=f"{arg} is a dual tensor"):
+            getattr(ssm, name)(**kw)
