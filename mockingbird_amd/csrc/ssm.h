@@ -100,11 +100,11 @@ __device__ __forceinline__ int lanes_prefix(int v) {  // inclusive, over the wav
   }
   return v;
 }
-// part < 0: no such tile.  Every lane of the wave calls it with the same tile.
-__device__ __forceinline__ Item item_of(const Rows& r, unsigned tile, int R) {
+// part < 0: no such tile.  Every lane of the wave calls it with the same tile.  less = 1: all but the last tile of each item are numbered.
+__device__ __forceinline__ Item item_of(const Rows& r, unsigned tile, int R, int less = 0) {
   Item it = {0, 0, 0, -1};
   if (!r.cu && !r.valid) {
-    const unsigned per = r.t > R ? (unsigned)(r.t + R - 1) / R : 1u;
+    const unsigned per = (r.t > R ? (unsigned)(r.t + R - 1) / R : 1u) - less;
     it.b = (int)(tile / per);
     it.part = (int)(tile - (unsigned)it.b * per);
     it.len = r.t;
@@ -116,7 +116,7 @@ __device__ __forceinline__ Item item_of(const Rows& r, unsigned tile, int R) {
     int first = 0, len = 0, parts = 0;
     if (i < r.batch) {
       len = rows_of(r, i, first);
-      parts = max(1, (len + R - 1) / R);
+      parts = max(1, (len + R - 1) / R) - less;
     }
     const int end = base + lanes_prefix(parts);
     const unsigned long long behind = __ballot(end > (int)tile);
@@ -132,15 +132,37 @@ __device__ __forceinline__ Item item_of(const Rows& r, unsigned tile, int R) {
   }
   return it;
 }
-// First tile of item b; every lane of the wave calls it with the same b.
-__device__ __forceinline__ int first_tile_of(const Rows& r, int b, int R) {
-  if (!r.cu && !r.valid) return b * (r.t > R ? (r.t + R - 1) / R : 1);
-  int sum = 0;
-  for (int i = (int)threadIdx.x & 63; i < b; i += 64) {
-    int first;
-    sum += max(1, (rows_of(r, i, first) + R - 1) / R);
+// The items of more than one tile, for calls whose tiles need a place in memory: together they have at most this many tiles in front of
+// their last ones, whatever the number of items.  (t > R)
+__host__ __device__ inline long long fronts_of(const Rows& r, int R) {
+  return r.cu ? (long long)r.t / R : (long long)r.batch * ((r.t + R - 1) / R - 1);
+}
+// The j-th of them (b < 0: there are not so many), its tiles, and how many tiles in front of last ones the items before it have.  Every lane
+// of the wave calls it with the same j.
+struct Long {
+  int b, parts, fronts;
+};
+__device__ __forceinline__ Long long_item(const Rows& r, int j, int R) {
+  if (!r.cu && !r.valid) {
+    const int parts = (r.t + R - 1) / R;
+    return {j, parts, j * (parts - 1)};
   }
-  return __builtin_amdgcn_readlane(lanes_prefix(sum), 63);
+  int items = 0, fronts = 0;
+  for (int i0 = 0; i0 < r.batch; i0 += 64) {
+    const int i = i0 + ((int)threadIdx.x & 63);
+    int first, parts = 1;
+    if (i < r.batch) parts = max(1, (rows_of(r, i, first) + R - 1) / R);
+    const int upto = items + lanes_prefix(parts > 1), before = fronts + lanes_prefix(parts - 1) - (parts - 1);
+    const unsigned long long behind = __ballot(upto > j);
+    if (behind) {
+      const int l = __builtin_amdgcn_readfirstlane(__ffsll((long long)behind) - 1);
+      return {i0 + l, __builtin_amdgcn_readlane(parts, l), __builtin_amdgcn_readlane(before, l)};
+    }
+    items = __builtin_amdgcn_readlane(upto, 63);
+    // (lists of overlapping rows could claim any number of tiles: 64 items have at most 2^30, and the sum stops there)
+    fronts = min(__builtin_amdgcn_readlane(before + (parts - 1), 63), (1 << 30) - 1);
+  }
+  return {-1, 0, 0};
 }
 
 // Slot of item b, or -1: outside the pool, or named by an earlier item as well (two updates of one state would race; the first wins).

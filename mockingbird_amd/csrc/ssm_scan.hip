@@ -65,43 +65,43 @@ __global__ __launch_bounds__(256) void selective_scan_step_kernel(const mb_selec
   }
 }
 
-// Between the two passes of a split call: every tile's own sum becomes the state in front of it.  4 elements per thread; the tiles are
-// read U ahead of the chain that runs over them.
+// Between the two passes of a split call: what every tile adds becomes the state in front of the next one.  A workgroup takes 1024 elements
+// of a head of the j-th item that is split, 4 per thread; the tiles are read U ahead of the chain that runs over them.
 __global__ __launch_bounds__(256) void selective_scan_join_kernel(const mb_selective_scan_args a, const Split sp) {
   constexpr int U = 4;
   const int elems = a.head_dim * a.d_state_dim, blocks = (elems + 1023) / 1024;
   const unsigned item_head = blockIdx.x / blocks;
   const int e = ((int)(blockIdx.x - item_head * blocks) * 256 + (int)threadIdx.x) * 4, n = elems - e;
-  const int b = (int)(item_head / a.heads), head = (int)(item_head - (unsigned)b * a.heads);
+  const int j = (int)(item_head / a.heads), head = (int)(item_head - (unsigned)j * a.heads);
+  const Rows rows = {a.d_cu_seqlens, a.d_valid, a.batch, a.t};
+  const Long it = long_item(rows, j, sp.seg);
+  if (it.b < 0) return;
   int slot = -1;
   if (a.d_state) {
-    slot = slot_of(a.d_slots, b, a.n_slots);
+    slot = slot_of(a.d_slots, it.b, a.n_slots);
     if (slot < 0) return;
   }
-  const Rows rows = {a.d_cu_seqlens, a.d_valid, a.batch, a.t};
-  int first;
-  const int parts = (rows_of(rows, b, first) + sp.seg - 1) / sp.seg;
-  if (parts <= 1) return;  // not split: its workgroups read and write the pool themselves
-  const long long tile = first_tile_of(rows, b, sp.seg);
-  if (n <= 0 || tile + parts > sp.tiles) return;  // (row numbers that overlap can claim more tiles than there are)
-  const bool keep = a.d_state && (!a.d_has_state || a.d_has_state[b]);
+  const bool keep = a.d_state && (!a.d_has_state || a.d_has_state[it.b]);
+  const int at = keep ? initial_at(sp, a.batch, it.b, it.fronts) : 0;
+  if (n <= 0 || at < 0 || it.fronts > sp.fronts - (it.parts - 1)) return;  // (row numbers that overlap can claim more tiles than there are)
   Vec<float, 4> h = load_some<float, 4>(a.d_state + slot * a.state_stride + (long long)head * elems + e, keep ? n : 0);
-  const long long step = (long long)a.heads * elems;
-  float* st = sp.state + (tile * a.heads + head) * (long long)elems + e;
-  const float* decay = sp.decay + tile * a.heads + head;
-  for (int k = 0; k < parts; k += U) {
+  const long long step = (long long)a.heads * elems, own_head = (long long)head * elems + e;
+  if (keep) store_some<float, 4>(sp.initial + at * step + own_head, h, n);
+  float* st = sp.state + it.fronts * step + own_head;
+  const float* decay = sp.decay + (long long)it.fronts * a.heads + head;
+  for (int k = 1; k < it.parts; k += U) {
     Vec<float, 4> own[U];
     float by[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {  // the last tile's own sum is not computed: nothing follows it
-      own[u] = load_some<float, 4>(st + u * step, k + u + 1 < parts ? n : 0);
-      by[u] = k + u + 1 < parts ? decay[(long long)u * a.heads] : 0.f;
+    for (int u = 0; u < U; ++u) {
+      own[u] = load_some<float, 4>(st + u * step, k + u < it.parts ? n : 0);
+      by[u] = k + u < it.parts ? decay[(long long)u * a.heads] : 0.f;
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      if (k + u < parts) store_some<float, 4>(st + u * step, h, n);
 #pragma unroll
       for (int i = 0; i < 4; ++i) h.v[i] = fmaf(h.v[i], by[u], own[u].v[i]);
+      if (k + u < it.parts) store_some<float, 4>(st + u * step, h, n);
     }
     st += U * step;
     decay += (long long)U * a.heads;
@@ -148,16 +148,18 @@ static int rows_per_tile(const mb_selective_scan_args& a) {
 }
 
 static size_t split_layout(const mb_selective_scan_args& a, void* base, Split* sp) {
+  *sp = {};
   sp->seg = rows_per_tile(a);
-  sp->state = sp->decay = nullptr;
-  sp->tiles = 0;
   if (!sp->seg) return 0;
   const Rows rows = {a.d_cu_seqlens, a.d_valid, a.batch, a.t};
-  const size_t tiles = (size_t)tiles_of(rows, sp->seg);
-  sp->tiles = (int)tiles;
+  const long long fronts = fronts_of(rows, sp->seg), initials = a.d_state ? (a.batch < fronts ? a.batch : fronts) : 0;
+  const size_t state = (size_t)a.heads * a.head_dim * a.d_state_dim;
+  sp->fronts = (int)fronts;
+  sp->initials = (int)initials;
   Arena ar(base, ~(size_t)0);
-  sp->state = ar.take<float>(tiles * a.heads * a.head_dim * a.d_state_dim);
-  sp->decay = ar.take<float>(tiles * a.heads);
+  sp->state = ar.take<float>(fronts * state);
+  sp->initial = ar.take<float>(initials * state);
+  sp->decay = ar.take<float>(fronts * a.heads);
   return align_up(ar.off, 256);
 }
 
@@ -223,7 +225,7 @@ static int run_scan(const mb_selective_scan_args* a, void* ws, size_t ws_bytes, 
   if (sp.seg) {
     const int rc = chunks(*a, sp, true, s);
     if (rc) return rc;
-    const long long grid = (long long)a->batch * a->heads * cdiv(a->head_dim * a->d_state_dim, 1024);
+    const long long grid = (long long)(a->batch < sp.fronts ? a->batch : sp.fronts) * a->heads * cdiv(a->head_dim * a->d_state_dim, 1024);
     MB_REQUIRE(grid < (1ll << 31), "selective_scan: %d items of %d heads are too many for one launch", a->batch, a->heads);
     hipLaunchKernelGGL(selective_scan_join_kernel, dim3((unsigned)grid), dim3(256), 0, s, *a, sp);
     MB_HIP(hipGetLastError());

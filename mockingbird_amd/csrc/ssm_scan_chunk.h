@@ -228,13 +228,21 @@ template <typename T, int V, int ROWS, int COLS, int THREADS> struct Stage {
   }
 };
 
-// Workspace of a call that is split along time: per tile of `seg` rows and head the state it adds, then the state in front of it, and its decay.
+// Workspace of a call that is split along time: for every tile of `seg` rows that has one behind it, in the order of items and rows, and every
+// head what it adds to the state, and its decay; the join puts the state in front of the next tile in the sum's place.  The state in front
+// of an item's first tile is in the pool, where the last tile leaves the new one: split items have a copy.
 struct Split {
-  float* state;  // [tiles][heads][head_dim][d_state]
-  float* decay;  // [tiles][heads]
-  int seg;       // rows of a tile, a multiple of L; 0: not split
-  int tiles;     // that the workspace has room for
+  float* state;   // [fronts][heads][head_dim][d_state]
+  float* initial; // [initials][heads][head_dim][d_state]
+  float* decay;   // [fronts][heads]
+  int seg;        // rows of a tile, a multiple of L; 0: not split
+  int fronts, initials;
 };
+// Where the copy of item b's state is; `before` tiles of earlier items have one behind them.  (-1, for lists of overlapping rows: there is none)
+__device__ __forceinline__ int initial_at(const Split& sp, int batch, int b, int before) {
+  if (batch <= sp.initials) return b;
+  return (unsigned)before < (unsigned)sp.initials ? before : -1;
+}
 
 __device__ __forceinline__ float exp2_of(float v) { return __builtin_amdgcn_exp2f(v); }
 // prefix sum over the 16 lanes of a row: shifts within the row bring in zeros
@@ -271,9 +279,9 @@ __global__ __launch_bounds__((ScanShape<T, NP, STATES>::THREADS), (ScanShape<T, 
 
   const Rows rows = {a.d_cu_seqlens, a.d_valid, a.batch, a.t};
   const int seg = sp.seg ? sp.seg : max(a.t, 1);
-  const Item it = item_of(rows, tile, seg);
+  const Item it = item_of(rows, tile, seg, STATES);  // nobody asks what the last part adds
   const int parts = max(1, (it.len + seg - 1) / seg);
-  if (it.part < 0 || it.part >= parts || (STATES && it.part == parts - 1)) return;  // nobody asks what the last part adds
+  if (it.part < 0 || it.part >= parts) return;
   int slot = -1;
   if (a.d_state) {
     slot = slot_of(a.d_slots, it.b, a.n_slots);
@@ -296,10 +304,15 @@ __global__ __launch_bounds__((ScanShape<T, NP, STATES>::THREADS), (ScanShape<T, 
   f32x4 h[NT];
   const long long head_state = (long long)head_dim * d_state;
   float* const pool = a.d_state ? a.d_state + slot * a.state_stride + head * head_state : nullptr;
-  float* const joined = sp.seg ? sp.state + ((long long)tile * a.heads + head) * head_state : nullptr;
   {
-    const float* from = parts > 1 ? joined : pool;  // an item of one part is not split
-    const bool keep = !STATES && mine && (parts > 1 || (pool && (!a.d_has_state || a.d_has_state[it.b])));
+    const float* from = pool;  // an item of one part is not split
+    const bool carried = !STATES && (it.part > 0 || (pool && (!a.d_has_state || a.d_has_state[it.b]))), keep = carried && mine;
+    if (carried && parts > 1) {
+      const int before = (int)tile - it.b;  // tiles in front of this one that have one behind them
+      const int at = it.part ? before - 1 : initial_at(sp, a.batch, it.b, before);
+      if (it.part ? (unsigned)at >= (unsigned)sp.fronts : at < 0) return;  // (lists of overlapping rows; all waves)
+      from = (it.part ? sp.state : sp.initial) + ((long long)at * a.heads + head) * head_state;
+    }
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         const int p = p0 + pw + li, n = nt / 2 * 32 + 8 * g + nt % 2 * 4;
@@ -659,7 +672,7 @@ __global__ __launch_bounds__((ScanShape<T, NP, STATES>::THREADS), (ScanShape<T, 
     return;
   }
   if (!mine) return;
-  float* const to = STATES ? joined : pool;
+  float* const to = STATES ? sp.state + ((long long)tile * a.heads + head) * head_state : pool;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const int p = p0 + pw + li, n = nt / 2 * 32 + 8 * g + nt % 2 * 4;
@@ -683,7 +696,7 @@ template <typename T, int NP, bool STATES, bool WHOLE> int launch_chunk(const mb
   const Rows rows = {a.d_cu_seqlens, a.d_valid, a.batch, a.t};
   const int per_group = a.heads / a.groups;
   const long long units = (long long)a.groups * cdiv(per_group, S::HB) * cdiv(a.head_dim, S::PB);
-  const long long grid = tiles_of(rows, sp.seg ? sp.seg : (a.t > 1 ? a.t : 1)) * units;
+  const long long grid = (STATES ? sp.fronts : tiles_of(rows, sp.seg ? sp.seg : (a.t > 1 ? a.t : 1))) * units;
   MB_REQUIRE(grid < (1ll << 31), "selective_scan: %d items of %d heads are too many for one launch", a.batch, a.heads);
   hipLaunchKernelGGL((selective_scan_chunk_kernel<T, NP, STATES, WHOLE>), dim3((unsigned)grid), dim3(S::THREADS), sizeof(typename S::Lds), s, a, sp);
   MB_HIP(hipGetLastError());
