@@ -95,16 +95,6 @@ __device__ __forceinline__ float value_of(const bf16x8& v, int i) {
   const u32x4 w = __builtin_bit_cast(u32x4, v);
   return __uint_as_float(i & 1 ? w[i >> 1] & 0xffff0000u : w[i >> 1] << 16);
 }
-// a NaN or infinity among 8 values
-__device__ __forceinline__ bool not_finite(const bf16x8& v) {
-  const u32x4 w = __builtin_bit_cast(u32x4, v);
-  typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
-  u16x2 top = {0, 0};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, w[i] & 0x7fff7fffu));
-  return top[0] >= 0x7f80 || top[1] >= 0x7f80;
-}
-
 // acc += a b over the plane pairs whose product is above 2^-8(K): K planes of the result are kept
 template <int QA, int QB, int K>
 __device__ __forceinline__ f32x4 mma(const bf16x8 (&a)[QA], const bf16x8 (&b)[QB], f32x4 acc) {
@@ -148,6 +138,7 @@ template <typename T, int NP, bool STATES> struct ScanShape {
   struct Lds : std::conditional<STATES, LdsStates, LdsY>::type {
     unsigned short b[R][L][NS], x[HB][R][L][PB];
     Head head[HEADS][HB];
+    int odd[HB][WPH];  // step sizes that the products cannot do
   };
   static constexpr int WAVES = (sizeof(Lds) <= 80 * 1024 ? 2 : 1) * THREADS / 256;  // per SIMD, of the workgroups that share a CU
 };
@@ -258,6 +249,126 @@ __device__ __forceinline__ double from_lane(double v, int lane) {
   return __builtin_bit_cast(double, ((unsigned long long)hi << 32) | lo);
 }
 
+// What a workgroup works on, from its number.
+template <typename T> struct Work {
+  const T *x, *b, *c;     // row 0 of the item: the first head's columns p0 .., the group's B and C
+  T* y;                   // this wave's columns
+  long long dt;
+  float* pool;            // this wave's head: its state, null without a pool
+  const float* from;      // and the state in front of the tile, if `carried`
+  unsigned tile;
+  int part, parts, t0, t1, p0, head0, live, head, columns;
+  bool carried, none;     // none: nothing to do
+};
+template <typename T, int NP, bool STATES, bool WHOLE>
+__device__ __forceinline__ Work<T> work_of(const mb_selective_scan_args& a, const Split& sp, unsigned block, int wave) {
+  typedef ScanShape<T, NP, STATES> S;
+  constexpr int HB = S::HB, PB = S::PB;
+  Work<T> w;
+  w.none = true;
+  const int head_dim = a.head_dim, d_state = WHOLE ? NP : a.d_state_dim;
+  const int per_group = a.heads / a.groups, hblocks = (per_group + HB - 1) / HB, pblocks = (head_dim + PB - 1) / PB;
+  const int units = a.groups * hblocks * pblocks;
+  w.tile = block / units;
+  int unit = (int)(block - w.tile * units);
+  w.p0 = unit % pblocks * PB;
+  unit /= pblocks;
+  const int hb = unit % hblocks, group = unit / hblocks;
+  w.head0 = group * per_group + hb * HB, w.live = WHOLE ? HB : min(HB, per_group - hb * HB);
+
+  const Rows rows = {a.d_cu_seqlens, a.d_valid, a.batch, a.t};
+  const int seg = sp.seg ? sp.seg : max(a.t, 1);
+  const Item it = item_of(rows, w.tile, seg, STATES);  // nobody asks what the last part adds
+  w.part = it.part, w.parts = max(1, (it.len + seg - 1) / seg);
+  if (it.part < 0 || it.part >= w.parts) return w;
+  int slot = -1;
+  if (a.d_state) {
+    slot = slot_of(a.d_slots, it.b, a.n_slots);
+    if (slot < 0) return w;
+  }
+  w.t0 = it.part * seg, w.t1 = min(it.len, w.t0 + seg);
+  const long long pad = a.d_cu_seqlens ? 0 : it.b;
+  w.x = (const T*)a.d_x + pad * a.x_bstride + it.row * a.x_rstride + (long long)w.head0 * head_dim + w.p0;
+  w.b = (const T*)a.d_b + pad * a.b_bstride + it.row * a.b_rstride + (long long)group * d_state;
+  w.c = (const T*)a.d_c + pad * a.c_bstride + it.row * a.c_rstride + (long long)group * d_state;
+  w.dt = pad * a.dt_bstride + it.row * a.dt_rstride;
+  w.head = w.head0 + min(wave % HB, w.live - 1);
+  w.columns = wave / HB * 16;  // p0 + these ..
+  w.y = (T*)a.d_y + pad * a.y_bstride + it.row * a.y_rstride + (long long)w.head * head_dim + w.p0 + w.columns;
+  const long long head_state = (long long)head_dim * d_state;
+  w.pool = a.d_state ? a.d_state + slot * a.state_stride + w.head * head_state : nullptr;
+  w.from = w.pool;  // an item of one part is not split
+  w.carried = !STATES && (it.part > 0 || (w.pool && (!a.d_has_state || a.d_has_state[it.b])));
+  if (w.carried && w.parts > 1) {
+    const int before = (int)w.tile - it.b;  // tiles in front of this one that have one behind them
+    const int at = it.part ? before - 1 : initial_at(sp, a.batch, it.b, before);
+    if (it.part ? (unsigned)at >= (unsigned)sp.fronts : at < 0) return w;  // (lists of overlapping rows; all waves)
+    w.from = (it.part ? sp.state : sp.initial) + ((long long)at * a.heads + w.head) * head_state;
+  }
+  w.none = false;
+  return w;
+}
+// h[2 q + e]: column p0 + columns + (lane & 15), state columns 32 q + 8 g + 4 e + i
+template <typename T, int NP, bool WHOLE> __device__ __forceinline__ void start_of(const Work<T>& w, int head_dim, int d_state, bool mine, int lane, f32x4 (&h)[NP / 16]) {
+#pragma unroll
+  for (int nt = 0; nt < NP / 16; ++nt) {
+    const int p = w.p0 + w.columns + (lane & 15), n = nt / 2 * 32 + 8 * (lane >> 4) + nt % 2 * 4;
+    const int left = w.carried && mine && (WHOLE || p < head_dim) ? (WHOLE ? 4 : d_state - n) : 0;
+    h[nt] = __builtin_bit_cast(f32x4, load_some<float, 4>(w.from + (long long)p * d_state + n, left));
+  }
+}
+
+// The tile again, row by row, each wave its own columns: where infinities, NaN or growth beyond fp32 keep the products from giving what the
+// recurrence gives.  (8192 rows, 64 heads of 64 x 128 bf16 with a NaN in every head: 1.9 ms instead of 0.13.)  It is called behind the
+// products, so nothing it needs is kept through them: the arguments are read anew from the kernel's own.
+template <typename T, int NP, bool STATES, bool WHOLE> __device__ __forceinline__ void walk_rows(f32x4 (&h)[NP / 16]) {
+  struct Args {
+    mb_selective_scan_args a;
+    Split sp;
+  };
+  typedef __attribute__((address_space(4))) const Args Given;
+  Given* given = (Given*)__builtin_amdgcn_kernarg_segment_ptr();
+  unsigned block = blockIdx.x;
+  asm volatile("" : "+s"(given), "+s"(block));
+  Args args;
+  __builtin_memcpy(&args, (const void*)given, sizeof(Args));
+  const mb_selective_scan_args& a = args.a;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = (int)threadIdx.x & 63, g = lane >> 4, li = lane & 15;
+  const Work<T> w = work_of<T, NP, STATES, WHOLE>(a, args.sp, block, wave);
+  const int d_state = WHOLE ? NP : a.d_state_dim, column = w.p0 + w.columns + li;
+  const bool there = WHOLE || column < a.head_dim;
+  start_of<T, NP, WHOLE>(w, a.head_dim, d_state, true, lane, h);
+  const T* x = w.x + (w.head - w.head0) * a.head_dim + w.columns + li;
+  const float A = a.d_a[w.head], skip = a.d_d ? a.d_d[w.head] : 0.f;
+  __threadfence();  // the answers below go behind those of the products
+  for (int t = w.t0; t < w.t1; ++t) {
+    const float d = step_size(a, w.dt + t * a.dt_rstride + w.head, w.head), decay = expf(d * A);
+    const float xv = there ? to_f32(x[t * a.x_rstride]) : 0.f, dx = d * xv;
+    float y = 0.f;
+    int fresh = lane;
+    asm volatile("" : "+v"(fresh));  // (masks and addresses by column are not worth registers of the loop)
+#pragma unroll
+    for (int nt = 0; nt < NP / 16; ++nt) {
+      const int n = nt / 2 * 32 + 8 * (fresh >> 4) + nt % 2 * 4;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int at = WHOLE ? n + r : min(n + r, d_state - 1);
+        const float bv = to_f32(w.b[t * a.b_rstride + at]), cv = STATES ? 0.f : to_f32(w.c[t * a.c_rstride + at]);
+        const float next = fmaf(h[nt][r], decay, dx * bv), sum = fmaf(next, cv, y);
+        const bool in = WHOLE || n + r < d_state;  // (0 * infinity)
+        h[nt][r] = in ? next : h[nt][r];
+        y = in ? sum : y;
+      }
+      if (nt % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // (not all loads of a row at once)
+    }
+    if constexpr (!STATES) {
+      y += __shfl_xor(y, 16, 64);
+      y += __shfl_xor(y, 32, 64);
+      if (there && g == 0) w.y[t * a.y_rstride + li] = from_f32<T>(fmaf(skip, xv, y));
+    }
+  }
+}
+
 // STATES: first pass of a split call, the state every tile adds to a zero state.  Otherwise y (and the final states).
 // WHOLE: head_dim is a multiple of 64, d_state is NP and the heads of a group are even: only rows can be missing.
 template <typename T, int NP, bool STATES, bool WHOLE>
@@ -267,59 +378,20 @@ __global__ __launch_bounds__((ScanShape<T, NP, STATES>::THREADS), (ScanShape<T, 
   extern __shared__ __attribute__((aligned(16))) char lds_raw[];
   typename S::Lds& m = *(typename S::Lds*)lds_raw;
 
-  const int head_dim = a.head_dim, d_state = WHOLE ? NP : a.d_state_dim;
-  const int per_group = a.heads / a.groups, hblocks = (per_group + HB - 1) / HB, pblocks = (head_dim + PB - 1) / PB;
-  const int units = a.groups * hblocks * pblocks;
-  const unsigned tile = blockIdx.x / units;
-  int unit = (int)(blockIdx.x - tile * units);
-  const int p0 = unit % pblocks * PB;
-  unit /= pblocks;
-  const int hb = unit % hblocks, group = unit / hblocks;
-  const int head0 = group * per_group + hb * HB, live = WHOLE ? HB : min(HB, per_group - hb * HB);
-
-  const Rows rows = {a.d_cu_seqlens, a.d_valid, a.batch, a.t};
-  const int seg = sp.seg ? sp.seg : max(a.t, 1);
-  const Item it = item_of(rows, tile, seg, STATES);  // nobody asks what the last part adds
-  const int parts = max(1, (it.len + seg - 1) / seg);
-  if (it.part < 0 || it.part >= parts) return;
-  int slot = -1;
-  if (a.d_state) {
-    slot = slot_of(a.d_slots, it.b, a.n_slots);
-    if (slot < 0) return;
-  }
-  const int t0 = it.part * seg, t1 = min(it.len, t0 + seg);
-  const long long pad = a.d_cu_seqlens ? 0 : it.b;
-  const T* xg = (const T*)a.d_x + pad * a.x_bstride + it.row * a.x_rstride + (long long)head0 * head_dim + p0;
-  const T* bg = (const T*)a.d_b + pad * a.b_bstride + it.row * a.b_rstride + (long long)group * d_state;
-  const T* cg = (const T*)a.d_c + pad * a.c_bstride + it.row * a.c_rstride + (long long)group * d_state;
-  const long long dtg = pad * a.dt_bstride + it.row * a.dt_rstride;
-
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = (int)threadIdx.x & 63, g = lane >> 4, li = lane & 15;
-  const int hh = wave % HB, quarter = wave / HB, head = head0 + min(hh, live - 1);
+  const Work<T> work = work_of<T, NP, STATES, WHOLE>(a, sp, blockIdx.x, wave);
+  if (work.none) return;
+  const int head_dim = a.head_dim, d_state = WHOLE ? NP : a.d_state_dim;
+  const unsigned tile = work.tile;
+  const int p0 = work.p0, head0 = work.head0, live = work.live, t0 = work.t0, t1 = work.t1, head = work.head, pw = work.columns, parts = work.parts;
+  const T *xg = work.x, *bg = work.b, *cg = work.c;
+  const long long dtg = work.dt;
+  T* const yg = work.y;
+  float* const pool = work.pool;
+  const int hh = wave % HB, quarter = wave / HB;
   const bool mine = hh < live;
-  const int pw = quarter * 16;  // this wave's columns p0 + pw ..
-  T* yg = (T*)a.d_y + pad * a.y_bstride + it.row * a.y_rstride + (long long)head * head_dim + p0 + pw;
-
-  // h[2 q + e]: column p0 + pw + li, state columns 32 q + 8 g + 4 e + i
   f32x4 h[NT];
-  const long long head_state = (long long)head_dim * d_state;
-  float* const pool = a.d_state ? a.d_state + slot * a.state_stride + head * head_state : nullptr;
-  {
-    const float* from = pool;  // an item of one part is not split
-    const bool carried = !STATES && (it.part > 0 || (pool && (!a.d_has_state || a.d_has_state[it.b]))), keep = carried && mine;
-    if (carried && parts > 1) {
-      const int before = (int)tile - it.b;  // tiles in front of this one that have one behind them
-      const int at = it.part ? before - 1 : initial_at(sp, a.batch, it.b, before);
-      if (it.part ? (unsigned)at >= (unsigned)sp.fronts : at < 0) return;  // (lists of overlapping rows; all waves)
-      from = (it.part ? sp.state : sp.initial) + ((long long)at * a.heads + head) * head_state;
-    }
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        const int p = p0 + pw + li, n = nt / 2 * 32 + 8 * g + nt % 2 * 4;
-        const int left = keep && (WHOLE || p < head_dim) ? (WHOLE ? 4 : d_state - n) : 0;
-        h[nt] = __builtin_bit_cast(f32x4, load_some<float, 4>(from + (long long)p * d_state + n, left));
-      }
-  }
+  start_of<T, NP, WHOLE>(work, head_dim, d_state, mine, lane, h);
 
   Stage<T, V, L, NP, THREADS> sb, sc;
   Stage<T, V, L, HB * PB, THREADS> sx;
@@ -361,11 +433,13 @@ __global__ __launch_bounds__((ScanShape<T, NP, STATES>::THREADS), (ScanShape<T, 
   // Everything of a chunk that depends on the step sizes alone, one lane per row.  Sums are fp64: a difference of two far prefixes keeps
   // its bits.  Exponents are base 2 from here on.
   float draw = 0.f;
+  bool odd = !STATES && !(fabsf(skips[hh]) < INFINITY);  // something that the products cannot do: see the end
   auto request_step = [&](int t) { draw = lane < min(t1 - t, L) ? step_raw(a, dtg + (t + lane) * a.dt_rstride + head) : 0.f; };
   auto scalars = [&](int t, int to) {
-    const float d = lane < min(t1 - t, L) ? step_of(a, draw, bias) : 0.f;
+    const bool row = lane < min(t1 - t, L);
+    const float d = row ? step_of(a, draw, bias) : 0.f;
     asm("" : "+s"(A));  // (its fp64 copy is not worth registers of the whole loop)
-    double s = (double)d * ((double)A * 1.4426950408889634);  // log2(e)
+    double s = row ? (double)d * ((double)A * 1.4426950408889634) : 0.0;  // log2(e)
     s += row_shifted<1>(s);
     s += row_shifted<2>(s);
     s += row_shifted<4>(s);
@@ -376,6 +450,8 @@ __global__ __launch_bounds__((ScanShape<T, NP, STATES>::THREADS), (ScanShape<T, 
       sum[j] = from_lane(s, 16 * j + 15);
       if (g == j) rest = sum[j] - s;  // to the end of the tile
     }
+    // prefixes that fp32 holds, growth that no product of factors takes out of it (NaN fails)
+    if (__any(!(s > -1e38 && s < 28.0 && rest < 28.0 && fabsf(d) < INFINITY))) m.odd[hh][quarter] = 1;
     typename S::Head& o = m.head[to][hh];
     if (lane < L) {
       const float hi = (float)s;
@@ -413,6 +489,7 @@ __global__ __launch_bounds__((ScanShape<T, NP, STATES>::THREADS), (ScanShape<T, 
   constexpr int HEADS = S::HEADS, FOUR = S::WPH;
   const bool stepper = mine && quarter == FOUR - 1;  // the wave of each head that does this, a chunk ahead of the others' products
   if (STATES ? mine : stepper) {
+    m.odd[hh][quarter] = 0;
     const int first = STATES ? quarter : 0, next = STATES ? FOUR : 1;
     request_step(t0 + first * L);
     scalars(t0 + first * L, first);
@@ -521,6 +598,10 @@ __global__ __launch_bounds__((ScanShape<T, NP, STATES>::THREADS), (ScanShape<T, 
         for (int j = 0; j < TT; ++j) {
           acc[j] *= hd.u[16 * j + li] * hd.front[j];
         }
+        float sum = 0.f;
+#pragma unroll
+        for (int j = 0; j < TT; ++j) sum += acc[j][0];  // (a C that is not finite spoils its row in every column)
+        odd |= !(fabsf(sum) < INFINITY);
       }
       meet();
     }
@@ -574,36 +655,9 @@ __global__ __launch_bounds__((ScanShape<T, NP, STATES>::THREADS), (ScanShape<T, 
       if (WHOLE) request(t + L, tid);
       __builtin_amdgcn_sched_barrier(0);
       if constexpr (!STATES) {
-        // 0 * NaN in the half of M that is zero would reach rows in front of the NaN: such elements are taken out of the product, and
-        // their column's rows from there on are set to NaN below
-        int bad = L;  // first such row of this lane's column
-        bool any = false;
         bf16x8 fx[L / 32][R];
 #pragma unroll
-        for (int k = 0; k < L / 32; ++k) {
-          read_x(k, fx[k]);
-          any |= not_finite(fx[k][0]);  // a raw value is finite if its first plane is
-        }
-        const bool poisoned = __any(any);
-        if (poisoned) {
-#pragma unroll
-          for (int k = 0; k < L / 32; ++k) {
-            u32x4 w[R];
-#pragma unroll
-            for (int q = 0; q < R; ++q) w[q] = __builtin_bit_cast(u32x4, fx[k][q]);
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-              if (!(fabsf(value_of(fx[k][0], i)) <= 3.4e38f)) {
-                bad = min(bad, 32 * k + (i < 4 ? 4 * g + i : 12 + 4 * g + i));
-#pragma unroll
-                for (int q = 0; q < R; ++q) w[q][i >> 1] &= i & 1 ? 0x0000ffffu : 0xffff0000u;
-              }
-#pragma unroll
-            for (int q = 0; q < R; ++q) fx[k][q] = __builtin_bit_cast(bf16x8, w[q]);
-          }
-          bad = min(bad, __shfl_xor(bad, 16, 64));
-          bad = min(bad, __shfl_xor(bad, 32, 64));
-        }
+        for (int k = 0; k < L / 32; ++k) read_x(k, fx[k]);
         const unsigned off_y = (li * (int)a.y_rstride + 4 * g) * (int)sizeof(T);
         // rows from the tile's end on are dropped by the descriptor's range check
         const __amdgpu_buffer_rsrc_t dy = tm_rsrc(yg + t * a.y_rstride, ((min(t1 - t, L) - 1) * (int)a.y_rstride + 16) * (int)sizeof(T));
@@ -630,13 +684,6 @@ __global__ __launch_bounds__((ScanShape<T, NP, STATES>::THREADS), (ScanShape<T, 
           if (j % 2) __builtin_amdgcn_sched_barrier(0);
         }
         // y^T tiles: row p = 4 g + i, column t = li
-        if (poisoned) {
-#pragma unroll
-          for (int j = 0; j < TT; ++j)
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-              if (16 * j + li >= __shfl(bad, 4 * g + r, 64)) acc[j][r] = __builtin_nanf("");
-        }
 #pragma unroll
         for (int j = 0; j < TT; ++j) {
           Vec<T, 4> o;
@@ -657,22 +704,32 @@ __global__ __launch_bounds__((ScanShape<T, NP, STATES>::THREADS), (ScanShape<T, 
     meet();
   }
 
-  if (STATES) {
-    if constexpr (STATES) {  // each wave has summed up its own chunks
-      if (mine && lane == 0) m.walked[hh][quarter] = walked;
-      meet();
-      if (stepper && lane == 0) {
-        double sum = 0.0;
-#pragma unroll
-        for (int i = 0; i < FOUR; ++i) sum += m.walked[hh][i];
-        sp.decay[(long long)tile * a.heads + head] = exp2_of((float)sum);
-      }
-    }
-  } else if (!pool || it.part != parts - 1) {
-    return;
+  if constexpr (STATES) {
+    if (mine && lane == 0) m.walked[hh][quarter] = walked;  // each wave has summed up its own chunks
+    meet();
   }
   if (!mine) return;
-  float* const to = STATES ? sp.state + ((long long)tile * a.heads + head) * head_state : pool;
+  if constexpr (STATES) {
+    if (stepper && lane == 0) {
+      double sum = 0.0;
+#pragma unroll
+      for (int i = 0; i < FOUR; ++i) sum += m.walked[hh][i];
+      sp.decay[(long long)tile * a.heads + head] = exp2_of((float)sum);
+    }
+  }
+  // Does this wave's result stand?  Products give NaN where the recurrence has an infinity, or a number: infinity - infinity between planes,
+  // 0 * NaN in the half of M that is zero, 0 * infinity between the factors of a decay.  What of that comes from x, B, dt or the state in
+  // front is in h for good, a C that is not finite was seen in C h, step sizes that the factors cannot do by the wave that made them.
+  float spoilt = 0.f;
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) spoilt = fmaf(h[nt][r], 0.f, spoilt);
+#pragma unroll
+  for (int i = STATES ? 0 : FOUR - 1; i < FOUR; ++i) odd |= m.odd[hh][i] != 0;
+  if (__any(odd || spoilt != 0.f)) walk_rows<T, NP, STATES, WHOLE>(h);
+  if (!STATES && (!pool || work.part != parts - 1)) return;
+  float* const to = STATES ? sp.state + ((long long)tile * a.heads + head) * ((long long)head_dim * d_state) : pool;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const int p = p0 + pw + li, n = nt / 2 * 32 + 8 * g + nt % 2 * 4;
