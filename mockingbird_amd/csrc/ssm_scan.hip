@@ -53,7 +53,8 @@ __global__ __launch_bounds__(256) void selective_scan_step_kernel(const mb_selec
       float s = 0.f;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        v[u].v[i] = fmaf(v[u].v[i], decay, dx * to_f32(br.v[i]));
+        const float next = fmaf(v[u].v[i], decay, dx * to_f32(br.v[i]));
+        v[u].v[i] = i < left ? next : 0.f;  // (0 * infinity in columns that are not there)
         s = fmaf(v[u].v[i], to_f32(cr.v[i]), s);
       }
       s = lanes_sum<LANES>(s);

@@ -110,3 +110,26 @@ def test_states_that_vanish_at_once(dtype, run):
         # products and sums of d_state + 2 terms, operands in planes of 2^-15 relative or fp32
         err = (dt.double() * size + c["skip"].double().abs())[..., None] * x.abs() * ((shape[2] + 8) * ref.U + (2.0 ** -15 if dtype is BF16 else 2.0 ** -21))
         same_values(y, want, ref.rounded(want, err, dtype), a)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("value", [INF, -INF, NAN])
+@pytest.mark.parametrize("what", ["x", "bm", "cm", "dt", "pool"])
+@pytest.mark.parametrize("shape", [(2, 64, 64, 1), (3, 20, 24, 1), (1, 5, 3, 1), (2, 16, 130, 2)])
+def test_single_tokens_with_an_infinity_or_nan(dtype, value, what, shape):
+    from test_ssm_gpu import gen, scan_inputs
+    from mockingbird_amd import ssm
+    h, p, n, g = shape
+    b = 4
+    r = gen(n)
+    x, dt, a, bm, cm, skip, bias = scan_inputs(r, (b,), h, p, n, g, dtype)
+    bm, cm, pool = bm.abs() + 0.125, cm.abs() + 0.125, r(b, h, p, n)
+    t = dict(x=x, bm=bm, cm=cm, dt=dt, pool=pool)[what]
+    t[(1,) + (0,) * (t.dim() - 1)] = value
+    t[(2,) + (-1,) * (t.dim() - 1)] = value
+    dpool = pool.cuda()
+    y = ssm.selective_scan_step(x.cuda(), dt.cuda(), a.cuda(), bm.cuda(), cm.cuda(), dpool, skip.cuda(), dt_bias=bias.cuda(), dt_softplus=True)
+    want, err, new, nerr = ref.scan(x, dt, a, bm, cm, skip, bias, True, None, [(i, 1) for i in range(b)], pool, list(range(b)), [True] * b)
+    err, nerr = torch.where(torch.isfinite(want), err, torch.zeros_like(err)), torch.where(torch.isfinite(new), nerr, torch.zeros_like(nerr))
+    same_values(y, want, ref.rounded(want, err, dtype), (what, "y"))
+    same_values(dpool, new, nerr + ref.HALF[F32] * new.abs() + ref.TINY[F32], (what, "state"))
