@@ -236,6 +236,7 @@ static inline int check_apart(const char* fn, const Span* s, int written, int al
 }
 
 __host__ __device__ static inline bool aligned(const void* p, size_t n) { return ((size_t)p & (n - 1)) == 0; }
+static inline bool launchable(long long workgroups, int threads) { return workgroups < (1ll << 31) && workgroups * threads < (1ll << 32); }
 static inline size_t size_of(int dtype) { return dtype == MB_F32 ? 4 : 2; }
 
 }  // namespace ssm

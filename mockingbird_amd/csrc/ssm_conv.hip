@@ -161,7 +161,7 @@ static int conv_apart(const char* name, const mb_causal_conv1d_args& a, bool ste
 template <typename T, int K> int launch_conv(const mb_causal_conv1d_args& a, bool step, hipStream_t s) {
   if (step) {
     const long long grid = (long long)a.batch * cdiv(a.channels, 64 * CONV_V);
-    MB_REQUIRE(grid < (1ll << 31), "causal_conv1d_step: %d items of %d channels are too many for one launch", a.batch, a.channels);
+    MB_REQUIRE(launchable(grid, 64), "causal_conv1d_step: %d items of %d channels are too many for one launch", a.batch, a.channels);
     if (const int rc = conv_apart("causal_conv1d_step", a, true)) return rc;
     hipLaunchKernelGGL((causal_conv1d_step_kernel<T, K>), dim3((unsigned)grid), dim3(64), 0, s, a);
   } else {
@@ -175,7 +175,7 @@ template <typename T, int K> int launch_conv(const mb_causal_conv1d_args& a, boo
     int R = 32;
     while (R > 8 && tiles_of(rows, R * (256 / cx)) * cdiv(nv, cx) < 2048) R /= 2;
     const long long grid = tiles_of(rows, R * (256 / cx)) * cdiv(nv, cx);
-    MB_REQUIRE(grid < (1ll << 31), "causal_conv1d: %d rows of %d channels are too many for one launch", a.t, a.channels);
+    MB_REQUIRE(launchable(grid, 256), "causal_conv1d: %d rows of %d channels are too many for one launch", a.t, a.channels);
     if (const int rc = conv_apart("causal_conv1d", a, false)) return rc;
     hipLaunchKernelGGL((causal_conv1d_kernel<T, K>), dim3((unsigned)grid), dim3(256), 0, s, a, cx, R);
   }

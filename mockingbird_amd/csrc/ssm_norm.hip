@@ -259,17 +259,18 @@ template <typename T, typename TR> int launch_norm(const mb_block_norm_args& a, 
   const bool wave = !grouped && nv <= 64;
   const bool whole = nv <= 4096 && (!grouped || (C / a.groups) % V == 0) && units < (1ll << 31);
   const size_t lds = whole && !wave && grouped ? ((size_t)nv + 2 * a.groups) * sizeof(float) : 0;
-#define MB_NORM(VPT, WAVE, GRID, THREADS) \
-  hipLaunchKernelGGL((block_norm_kernel<T, TR, VPT, WAVE>), dim3((unsigned)(GRID)), dim3(THREADS), lds, s, a, parts, units)
+  const int vpt = nv <= (units < 512 ? 1024 : 256) ? 1 : nv <= 2048 ? 2 : 4, threads = wave || !whole ? 256 : (cdiv(nv, vpt) + 63) / 64 * 64;
+  const long long grid = !whole ? a.rows : wave ? (units + 3) / 4 : units;
+  MB_REQUIRE(launchable(grid, threads), "block_norm: %lld rows of %d channels are too many for one launch", a.rows, a.channels);
+#define MB_NORM(VPT, WAVE) hipLaunchKernelGGL((block_norm_kernel<T, TR, VPT, WAVE>), dim3((unsigned)grid), dim3(threads), lds, s, a, parts, units)
   if (whole && wave) {
-    MB_NORM(1, true, (units + 3) / 4, 256);
+    MB_NORM(1, true);
   } else if (whole) {
-    const int vpt = nv <= (units < 512 ? 1024 : 256) ? 1 : nv <= 2048 ? 2 : 4, threads = (cdiv(nv, vpt) + 63) / 64 * 64;
-    if (vpt == 1) MB_NORM(1, false, units, threads);
-    else if (vpt == 2) MB_NORM(2, false, units, threads);
-    else MB_NORM(4, false, units, threads);
+    if (vpt == 1) MB_NORM(1, false);
+    else if (vpt == 2) MB_NORM(2, false);
+    else MB_NORM(4, false);
   } else {
-    hipLaunchKernelGGL((block_norm_row_kernel<T, TR>), dim3((unsigned)a.rows), dim3(256), (size_t)2 * a.groups * sizeof(float), s, a);
+    hipLaunchKernelGGL((block_norm_row_kernel<T, TR>), dim3((unsigned)grid), dim3(threads), (size_t)2 * a.groups * sizeof(float), s, a);
   }
 #undef MB_NORM
   MB_HIP(hipGetLastError());

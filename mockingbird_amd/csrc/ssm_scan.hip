@@ -133,7 +133,7 @@ template <typename T, int LANES> int launch_step(const mb_selective_scan_args& a
   // few requests: a head's rows are dealt to more workgroups, down to one pass each, until two fit every CU
   while (pb > ROWS && (long long)a.batch * a.heads * ((a.head_dim + pb - 1) / pb) < 512) pb = (pb / ROWS + 1) / 2 * ROWS;
   const long long grid = (long long)a.batch * a.heads * ((a.head_dim + pb - 1) / pb);
-  MB_REQUIRE(grid < (1ll << 31), "selective_scan_step: %d items of %d heads are too many for one launch", a.batch, a.heads);
+  MB_REQUIRE(launchable(grid, 256), "selective_scan_step: %d items of %d heads are too many for one launch", a.batch, a.heads);
   hipLaunchKernelGGL((selective_scan_step_kernel<T, LANES>), dim3((unsigned)grid), dim3(256), 0, s, a, pb);
   MB_HIP(hipGetLastError());
   return MB_OK;
@@ -245,7 +245,7 @@ static int run_scan(const mb_selective_scan_args* a, void* ws, size_t ws_bytes, 
     const int rc = chunks(*a, sp, true, s);
     if (rc) return rc;
     const long long grid = (long long)(a->batch < sp.fronts ? a->batch : sp.fronts) * a->heads * cdiv(a->head_dim * a->d_state_dim, 1024);
-    MB_REQUIRE(grid < (1ll << 31), "selective_scan: %d items of %d heads are too many for one launch", a->batch, a->heads);
+    MB_REQUIRE(launchable(grid, 256), "selective_scan: %d items of %d heads are too many for one launch", a->batch, a->heads);
     hipLaunchKernelGGL(selective_scan_join_kernel, dim3((unsigned)grid), dim3(256), 0, s, *a, sp);
     MB_HIP(hipGetLastError());
   }

@@ -741,6 +741,11 @@ __global__ __launch_bounds__((ScanShape<T, NP, STATES>::THREADS), (ScanShape<T, 
 template <typename T, int NP, bool STATES, bool WHOLE> int launch_chunk(const mb_selective_scan_args& a, const Split& sp, hipStream_t s) {
   typedef ScanShape<T, NP, STATES> S;
   static_assert(sizeof(typename S::Lds) <= 160 * 1024, "a chunk has to fit LDS");
+  const Rows rows = {a.d_cu_seqlens, a.d_valid, a.batch, a.t};
+  const int per_group = a.heads / a.groups;
+  const long long units = (long long)a.groups * cdiv(per_group, S::HB) * cdiv(a.head_dim, S::PB);
+  const long long grid = (STATES ? sp.fronts : tiles_of(rows, sp.seg ? sp.seg : (a.t > 1 ? a.t : 1))) * units;
+  MB_REQUIRE(launchable(grid, S::THREADS), "selective_scan: %d items of %d heads are too many for one launch", a.batch, a.heads);
   static std::atomic<unsigned long long> attr_done{0};  // per device: the attribute belongs to the function on the current device
   int dev = 0;
   MB_HIP(hipGetDevice(&dev));
@@ -750,11 +755,6 @@ template <typename T, int NP, bool STATES, bool WHOLE> int launch_chunk(const mb
                                hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
     attr_done.fetch_or(bit, std::memory_order_release);
   }
-  const Rows rows = {a.d_cu_seqlens, a.d_valid, a.batch, a.t};
-  const int per_group = a.heads / a.groups;
-  const long long units = (long long)a.groups * cdiv(per_group, S::HB) * cdiv(a.head_dim, S::PB);
-  const long long grid = (STATES ? sp.fronts : tiles_of(rows, sp.seg ? sp.seg : (a.t > 1 ? a.t : 1))) * units;
-  MB_REQUIRE(grid < (1ll << 31), "selective_scan: %d items of %d heads are too many for one launch", a.batch, a.heads);
   hipLaunchKernelGGL((selective_scan_chunk_kernel<T, NP, STATES, WHOLE>), dim3((unsigned)grid), dim3(S::THREADS), sizeof(typename S::Lds), s, a, sp);
   MB_HIP(hipGetLastError());
   return MB_OK;

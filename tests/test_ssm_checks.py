@@ -175,3 +175,24 @@ def test_forward_mode_derivatives_are_refused(cuda, lib, i, arg, grad):
         kw[arg] = forward_ad.make_dual(kw[arg], torch.ones_like(kw[arg]))
         with pytest.raises(_lib.MbHipError, match=f"{arg} is a dual tensor"):
             getattr(ssm, name)(**kw)
+
+
+def test_launches_beyond_the_hardware_are_refused_by_name(lib):
+    """A launch has less than 2^32 threads."""
+    from mockingbird_amd import _lib
+    if torch.cuda.is_available():
+        pytest.skip("a call that is not refused would be launched on addresses that are none")
+    rows = 1 << 24
+    norm = _lib.BlockNormArgs(d_x=1 << 60, d_sum=1 << 61, rows=rows, channels=4096, groups=1, norm=1, dtype=_lib.MB_BF16, res_dtype=_lib.MB_BF16, x_rstride=4096,
+                              sum_rstride=4096, eps=1e-5, res_scale=1.0)
+    scan = _lib.SelectiveScanArgs(d_x=1 << 56, d_y=1 << 57, d_dt=1 << 58, d_b=1 << 59, d_c=1 << 60, d_a=256, dtype=_lib.MB_BF16, dt_dtype=_lib.MB_BF16, batch=rows, t=1,
+                                  heads=2, head_dim=64, groups=1, d_state_dim=64, dt_min=0.0, dt_max=1.0)
+    step = _lib.SelectiveScanArgs(d_x=1 << 56, d_y=1 << 57, d_dt=1 << 58, d_b=1 << 59, d_c=1 << 60, d_a=256, d_state=1 << 61, n_slots=rows, dtype=_lib.MB_BF16,
+                                  dt_dtype=_lib.MB_BF16, batch=rows, heads=2, head_dim=64, groups=1, d_state_dim=64, dt_min=0.0, dt_max=1.0)
+    conv = _lib.CausalConv1dArgs(d_x=1 << 60, d_y=1 << 61, d_w=256, dtype=_lib.MB_BF16, batch=rows, t=1, channels=64, ksize=4)
+    conv_step = _lib.CausalConv1dArgs(d_x=1 << 60, d_y=1 << 61, d_w=256, d_state=1 << 62, n_slots=1 << 27, dtype=_lib.MB_BF16, batch=1 << 27, channels=64, ksize=4)
+    for name, call in dict(block_norm=lambda: lib.mb_block_norm(norm, None), selective_scan=lambda: lib.mb_selective_scan(scan, None, 0, None),
+                           selective_scan_step=lambda: lib.mb_selective_scan_step(step, None), causal_conv1d=lambda: lib.mb_causal_conv1d(conv, None),
+                           causal_conv1d_step=lambda: lib.mb_causal_conv1d_step(conv_step, None)).items():
+        assert call() == -1, name
+        assert "too many" in lib.mb_last_error().decode() and name in lib.mb_last_error().decode()
