@@ -74,3 +74,26 @@ def test_row_numbers_in_no_order_stay_inside(cuda, lib, seed):
     ssm.selective_scan(x, dt, a, bm, cm, skip, dt_bias=bias, dt_softplus=True, cu_seqlens=cu, state=pools[1:b + 1], out=wide[64:t + 64])
     torch.cuda.synchronize()
     assert (wide[:64] == 7.0).all() and (wide[t + 64:] == 7.0).all() and (pools[[0, b + 1]] == 3.0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("shape,batch,t", [((2, 64, 64, 1), 3, 700), ((3, 20, 24, 3), 2, 641), ((2, 64, 64, 1), 1, 321)])
+def test_padded_requests_of_one_length(cuda, lib, dtype, shape, batch, t):
+    """[batch, t, ...] without lengths, split along time, with and without states to start from."""
+    import ssm_reference as ref
+    from test_ssm_gpu import PLANES, flat, gen, pool_of, scan_inputs, slot_args
+    from mockingbird_amd import ssm
+    h, p, n, g = shape
+    assert workspace(lib, batch, t, False, h, p, n, g, {F32: 0, F16: 1, BF16: 3}[dtype]) > 0
+    r = gen(t)
+    x, dt, a, bm, cm, skip, bias = scan_inputs(r, (batch, t), h, p, n, g, dtype)
+    a = a * 0.1
+    seqs = ref.sequences([t] * batch, False, t)
+    pool, slots, has = pool_of(batch, (h, p, n), seqs, r, F32)
+    dpool = pool.cuda()
+    y = ssm.selective_scan(x.cuda(), dt.cuda(), a.cuda(), bm.cuda(), cm.cuda(), skip.cuda(), dt_bias=bias.cuda(), dt_softplus=True, state=dpool,
+                           **slot_args(slots, has))
+    want, err, new, nerr = ref.scan(flat(x, 2), flat(dt, 1), a, flat(bm, 2), flat(cm, 2), skip, bias, True, None, seqs, pool, slots, has, PLANES[dtype])
+    ref.check(flat(y, 2), want, ref.rounded(want, err, dtype), "y")
+    ref.check(dpool.cpu()[slots], new[slots], nerr[slots] + ref.HALF[F32] * new[slots].abs() + ref.TINY[F32], "state")
