@@ -22,7 +22,7 @@ __device__ __forceinline__ float block_sum(float v, float* part, int waves) {  /
 // One pass over memory: a row (or, where the first norm's groups are all that couples channels, one group of a row) is held in
 // registers, VPT vectors of 16 bytes per thread, by one wave (WAVE: up to 64 vectors, no barrier, 4 rows per workgroup) or one workgroup.
 // Statistics are two-pass (mean, then centred squares) in fp32.  Memory-bound: 16384 x 4096 bf16 in 8 gated groups (6 bytes per element)
-// takes 79 us, 5.1 TB/s, a large copy's rate; 8192 x 2048 bf16 with an fp32 residual (12 bytes) 38 us, 5.3 TB/s.
+// takes 86 us (at best 83), 4.7 TB/s, of 5.2 that a large copy reaches; 8192 x 2048 bf16 with an fp32 residual (12 bytes) 36 us, warm.
 // Why these widths: a wave with 4 vectors per lane holds 162 registers and ran that second case in 46 us; one vector per thread in
 // workgroups of more than 256 threads loses to two (3001 fp16 channels: 46 and 41 us) unless there are too few rows to fill the chip
 // (64 rows of 4096: 6.2 and 7.6 us); four vectors of a 16-bit type spill at 1024 threads, so they begin where two end.
@@ -182,7 +182,9 @@ __global__ __launch_bounds__(WAVE ? 256 : 1024) void block_norm_kernel(const mb_
   }
 }
 
-// Any width, groups of any size: one workgroup per row, three passes over the row.
+// Any width, groups of any size: one workgroup per row, three passes over the row, element by element.  Rows that registers hold come here
+// only for groups that no number of 16-byte vectors fills, with a next norm: 8192 x 2000 bf16, 4 groups, gate, fp32 residual, next norm take
+// 152 us where 2048 channels take 41.
 template <typename T, typename TR>
 __global__ __launch_bounds__(256) void block_norm_row_kernel(const mb_block_norm_args a) {
   constexpr bool FAST = sizeof(T) == 2;

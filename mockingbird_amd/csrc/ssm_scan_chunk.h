@@ -11,21 +11,25 @@
 // order: x^T by transposing reads of rows 4 g + i and 16 + 4 g + i; for C h the state's rows are numbered so that the order is C's own
 // (tile 2 q holds columns 32 q + 8 g + i, tile 2 q + 1 those 4 further on).
 //
-// What bounds it: per wave and chunk 97 matrix instructions and about 570 vector ones, most of which split h, M and c x into planes, take 28 %
-// and 40 % of the time of their pipes and overlap by half at best; the rest is the order of a chunk -- step sizes, G, M, M x, three meetings of
-// the waves (39 % of their time is waiting; 60 vector instructions fewer gave 1 %).  Hence: M is formed once per head and goes through LDS; two
-// workgroups of 8 waves fit a CU (78 KB of LDS, 128 registers, nothing spilled -- a reload waits for the loads in flight in front of it),
-// so that one's products run while the other waits; the terms of the step sizes are a chunk ahead; the conversion of the next operand
-// stands between the products of this one.  Four waves of 32 columns read LDS half as often and are no faster (8192 rows, 64 heads of
-// 64 x 128: 149 and 146 us), one workgroup of four heads neither, nor the second pass adding up the tiles in front of its own instead of a
-// join (156 and 137 us).
-// Measured, 8192 rows x 64 heads of 64 columns, 128 states, bf16: 80 us this pass, 41 us the states' pass, 13 us the join between them, of
-// 28 us that its bytes take at a large copy's rate.  Planes less would save 9 us (h and M in one) and 10 us (c x in two) of it.
+// What bounds it: per wave and chunk 97 matrix instructions and about 580 vector ones, most of which split h, M and c x into planes, take 25 %
+// and 38 % of the time of their pipes and overlap by half at best; the rest is the order of a chunk -- step sizes, G, M, M x, three meetings of
+// the waves (41 % of their time is waiting; 60 vector instructions fewer gave 1 %).  Hence: M is formed once per head and goes through LDS; two
+// workgroups of 8 waves fit a CU (78 KB of LDS, 128 registers; nothing spilled at 128 states -- a reload waits for the loads in flight in
+// front of it -- while bf16 at 256 states spills 15 registers, and sizes that are not whole tiles 6 at 128 states and 86 at 256), so that one's
+// products run while the other waits; the terms of the step sizes are a chunk ahead; the conversion of the next operand stands between the
+// products of this one.  Four waves of 32 columns read LDS half as often and are no faster (8192 rows, 64 heads of 64 x 128: 149 and 146 us),
+// one workgroup of four heads neither, nor the second pass adding up the tiles in front of its own instead of a join (156 and 137 us).
+// Measured, 8192 rows x 64 heads of 64 columns, 128 states, bf16: 86 us this pass (at best 78), 43 (40) the states' pass, 14 the join between
+// them, of 28 us that its bytes take at a large copy's rate.  Planes less would save 9 us (h and M in one) and 10 us (c x in two) of it.
+// Sizes that are not whole tiles load and lay down in one go, nothing ahead: 48 heads of 96 x 100 take 219 us where 64 of 64 x 128 take 137;
+// narrow heads and small states are computed as 64 columns and states: 64 heads of 32 x 16 take 98 us.
 //
 // Precision.  Every sum, the state and all exponents are fp32 (prefix sums over a chunk: fp64, so that differences of far rows keep
 // their bits).  Operands are bf16 planes: a raw value is exact in 1 (bf16), 2 (fp16) or 3 (fp32) planes; computed operands are split as
 // well -- M and h into two planes (2^-17 relative; three for fp32 calls) since y is rounded to 2^-9 or 2^-12 behind them, c_s x_s of the
-// state into three, because the state is an fp32 result.  Products of planes below the last kept one are left out.
+// state into three, because the state is an fp32 result.  Products of planes below the last kept one are left out: up to 2^-18 of each term
+// of G, C h and M x in fp16 calls, 2^-25 in fp32 ones.  So a 16-bit y is a plain fp32 evaluation's up to single last places (in 0.1 % of a
+// bf16 result, 1 % of an fp16 one) unless its terms cancel to less than about 2^-8 (bf16) or 2^-5 (fp16) of their size, and the state is an fp32 evaluation's.
 #pragma once
 #include <atomic>
 #include "ssm.h"
