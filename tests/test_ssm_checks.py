@@ -196,3 +196,40 @@ def test_launches_beyond_the_hardware_are_refused_by_name(lib):
                            causal_conv1d_step=lambda: lib.mb_causal_conv1d_step(conv_step, None)).items():
         assert call() == -1, name
         assert "too many" in lib.mb_last_error().decode() and name in lib.mb_last_error().decode()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("i", range(6))
+def test_calls_while_another_device_is_current(cuda, lib, monkeypatch, i):
+    """The way that a call takes when its tensors are not on the current device (which is said to be another one here)."""
+    from mockingbird_amd import ssm
+    name, spec = arguments()[i]
+    r = torch.Generator().manual_seed(i)
+    kw = {k: torch.randn(shape, generator=r).cuda() if dtype is F32 else torch.ones(shape, dtype=dtype, device="cuda") for k, (shape, dtype) in spec.items()}
+    if "cu_seqlens" in kw:
+        kw["cu_seqlens"].copy_(torch.tensor([0, 2, T]))
+    if "slots" in kw:
+        kw["slots"].copy_(torch.arange(kw["slots"].numel()))
+    if "lengths" in kw:
+        kw["lengths"].fill_(T // 2)
+    if "A" in kw:
+        kw["A"].abs_().neg_()
+    if name == "block_norm":
+        kw["norm"], kw["next_norm"] = "layer", "rms"
+    other = {k: v.clone() if torch.is_tensor(v) else v for k, v in kw.items()}
+    want = getattr(ssm, name)(**kw)
+    entered = []
+
+    class Entered(torch.cuda.device):
+        def __enter__(self):
+            entered.append(self.idx)
+            return super().__enter__()
+
+    monkeypatch.setattr(ssm, "_device", lambda: torch.cuda.device_count())
+    monkeypatch.setattr(torch.cuda, "device", Entered)
+    got = getattr(ssm, name)(**other)
+    assert entered == [0]
+    for a, b in zip(want if isinstance(want, tuple) else (want,), got if isinstance(got, tuple) else (got,)):
+        assert torch.equal(a, b)
+    if "state" in kw:
+        assert torch.equal(kw["state"], other["state"])
