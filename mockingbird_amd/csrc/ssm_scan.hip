@@ -109,14 +109,15 @@ __global__ __launch_bounds__(256) void selective_scan_join_kernel(const mb_selec
 #pragma unroll
     for (int i = 0; i < 4; ++i) spoilt |= isnan(h.v[i]);
     if (__builtin_expect(spoilt, 0)) {
-      // The decay of a whole tile can leave fp32 where no row's does: what is infinite stays so beside a zero, a zero beside an infinity.
+      // The decay of a whole tile can leave fp32 where no row's does (-0: one does): what is infinite stays so beside a zero, a zero beside an
+      // infinity.
       h = was;
 #pragma unroll
       for (int u = 0; u < U; ++u) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           float v = h.v[i] * by[u];
-          if (isnan(v) && !isnan(h.v[i]) && !isnan(by[u])) v = h.v[i];
+          if (isnan(v) && !isnan(h.v[i]) && !isnan(by[u]) && __float_as_uint(by[u]) != 0x80000000u) v = h.v[i];
           h.v[i] = v + own[u].v[i];
         }
         if (k + u < it.parts) store_some<float, 4>(st + u * step, h, n);

@@ -229,7 +229,7 @@ template <typename T, int V, int ROWS, int COLS, int THREADS> struct Stage {
 struct Split {
   float* state;   // [fronts][heads][head_dim][d_state]
   float* initial; // [initials][heads][head_dim][d_state]
-  float* decay;   // [fronts][heads]
+  float* decay;   // [fronts][heads]; -0: a row's own decay is zero, 0: only their product is
   int seg;        // rows of a tile, a multiple of L; 0: not split
   int fronts, initials;
 };
@@ -444,6 +444,7 @@ __global__ __launch_bounds__((ScanShape<T, NP, STATES>::THREADS), (ScanShape<T, 
     const float d = row ? step_of(a, draw, bias) : 0.f;
     asm("" : "+s"(A));  // (its fp64 copy is not worth registers of the whole loop)
     double s = row ? (double)d * ((double)A * 1.4426950408889634) : 0.0;  // log2(e)
+    if (STATES && __any(s < -150.0)) walked = -INFINITY;  // a row whose own decay is zero
     s += row_shifted<1>(s);
     s += row_shifted<2>(s);
     s += row_shifted<4>(s);
@@ -718,7 +719,7 @@ __global__ __launch_bounds__((ScanShape<T, NP, STATES>::THREADS), (ScanShape<T, 
       double sum = 0.0;
 #pragma unroll
       for (int i = 0; i < FOUR; ++i) sum += m.walked[hh][i];
-      sp.decay[(long long)tile * a.heads + head] = exp2_of((float)sum);
+      sp.decay[(long long)tile * a.heads + head] = sum == -INFINITY ? -0.f : exp2_of((float)sum);
     }
   }
   // Does this wave's result stand?  Products give NaN where the recurrence has an infinity, or a number: infinity - infinity between planes,

@@ -133,3 +133,18 @@ def test_single_tokens_with_an_infinity_or_nan(dtype, value, what, shape):
     err, nerr = torch.where(torch.isfinite(want), err, torch.zeros_like(err)), torch.where(torch.isfinite(new), nerr, torch.zeros_like(nerr))
     same_values(y, want, ref.rounded(want, err, dtype), (what, "y"))
     same_values(dpool, new, nerr + ref.HALF[F32] * new.abs() + ref.TINY[F32], (what, "state"))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("run", [2, 3])
+def test_an_infinity_meets_a_decay_of_zero(dtype, run):
+    """0 * infinity in a row is NaN, whichever tile the row is in; decays that are zero only together leave the infinity."""
+    shape, lens = RUNS[run]
+    for gone in (None, lens[0] - 40, lens[0] // 2, 200):
+        c = case(70 + run, shape, lens, dtype, True)
+        c["a"], c["bias"] = c["a"] * 30 - 2.0, None
+        c["dt"] = c["dt"].float().abs() * 0.5 + 0.5  # (16 rows decay by 2^-23 and more, a tile by less than fp32 has)
+        c["x"][20, 0, 5] = INF
+        if gone is not None:
+            c["dt"][gone] = 1e5
+        run_and_check(c, dtype, ("zero", gone), softplus=False)
